@@ -65,6 +65,14 @@ class KvBlock(ctypes.Structure):
                 ("rows", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
+class Pages(ctypes.Structure):
+    """cqkv_pages: the page table and prefix sums of a packed batch over a page pool."""
+    _fields_ = [("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+                ("cu_seqlens", ctypes.c_void_p), ("batch", ctypes.c_int32),
+                ("max_pages", ctypes.c_int32), ("n_pages", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
 _lib = None
 
 
@@ -133,6 +141,16 @@ def lib() -> ctypes.CDLL:
         L.cqkv_dequantize_workspace_bytes.argtypes = [SP, i32, i32, i32]
         L.cqkv_dequantize_workspace_bytes.restype = sz
         L.cqkv_dequantize_rows.argtypes = [SP, i32, i32, i32, i32, P, i32, I64P, P, sz, P]
+        PP = ctypes.POINTER(Pages)
+        i64 = ctypes.c_int64
+        L.cqkv_paged_append.argtypes = [SP, SP, PP, P, P, I64P, P, I64P, i32, i32, P]
+        L.cqkv_paged_rope_append.argtypes = [SP, SP, PP, P, P, I64P, P, I64P, P, I64P, i32, i32, i32,
+                                             P, P, i32, i32, i32, P, i64, P, P, I64P, P]
+        L.cqkv_paged_dequantize.argtypes = [SP, PP, P, i32, P, i32, I64P, P]
+        L.cqkv_paged_attention_workspace_bytes.argtypes = [SP] + [i32] * 7
+        L.cqkv_paged_attention_workspace_bytes.restype = sz
+        L.cqkv_paged_attention.argtypes = [P, I64P, i32, SP, SP, PP, P, i32, i32, i32, i32, f32, i32,
+                                           i32, f32, P, i32, P, I64P, P, sz, P]
         L.cqkv_last_error.restype = ctypes.c_char_p
         L.cqkv_version.restype = ctypes.c_char_p
         _lib = L
@@ -151,6 +169,8 @@ EXPORTED = ["cqkv_codes_plane_bytes", "cqkv_scales_plane_bytes", "cqkv_quant_app
             "cqkv_rows_export", "cqkv_side_copy", "cqkv_turbo_codebook", "cqkv_turbo_signs",
             "cqkv_qjl_matrix", "cqkv_rotation_matrix", "cqkv_resolve_rotation",
             "cqkv_dequantize_workspace_bytes", "cqkv_dequantize_rows",
+            "cqkv_paged_append", "cqkv_paged_rope_append", "cqkv_paged_dequantize",
+            "cqkv_paged_attention", "cqkv_paged_attention_workspace_bytes",
             "cqkv_last_error",
             "cqkv_version"]
 
@@ -736,6 +756,210 @@ def flash_attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         window_right,
         softcap, al, al_bs, _ptr(cu_seqlens_q), _ptr(cu_seqlens_k), total_q, total_k, None, None,
         0, _ptr(ws), 0 if ws is None else ws.numel(), _stream(q.device)))
+    return out
+
+
+# ------------------------------------------------------------------------------------------
+# page pools: many sequences of different lengths in pages of one pool
+# ------------------------------------------------------------------------------------------
+# A pool is a key side and a value side whose batch counts pages and whose capacity is the page size
+# (a power of two from 32 on): CacheSide.empty(fmt, is_value, n_pages, kv_heads, head_dim, page_size,
+# device), formats FP8, MXFP8 and MXFP4, the same on both sides, unrotated. Tokens are packed: row i
+# belongs to the sequence b with cu_seqlens[b] <= i < cu_seqlens[b + 1]. page_table (batch, max_pages)
+# int32; ids outside the pool are holes (appends there are dropped, they read back as zeros, their keys
+# are masked).
+_I64x2 = ctypes.c_int64 * 2
+
+
+def _strides2(t: torch.Tensor) -> ctypes.Array:
+    return _I64x2(t.stride(0), t.stride(1))
+
+
+def _int_array(t: torch.Tensor, what: str, n: int | None, device: torch.device) -> int:
+    if t.device != device or t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 1:
+        raise CqkvError(ERR_ARG, f"{what} must be a contiguous 1-D int32 tensor on {device}")
+    if n is not None and t.numel() != n:
+        raise CqkvError(ERR_ARG, f"{what} has {t.numel()} entries, not {n}")
+    return t.data_ptr()
+
+
+def _pages(side: CacheSide, page_table: torch.Tensor, cu_seqlens: torch.Tensor) -> Pages:
+    dev = side.codes.device
+    _need_gpu(side.codes, "the page pool")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev:
+        raise CqkvError(ERR_ARG, f"page_table must be a (batch, max_pages) int32 tensor on {dev}")
+    b, n = page_table.shape
+    if n > 1 and page_table.stride(1) != 1:
+        raise CqkvError(ERR_ARG, "page_table needs contiguous rows")
+    return Pages(page_table.data_ptr(), page_table.stride(0),
+                 _int_array(cu_seqlens, "cu_seqlens", b + 1, dev), b, n, side.batch, 0)
+
+
+def _packed(t: torch.Tensor, what: str, side: CacheSide, heads: int | None = None) -> None:
+    """A packed row tensor (total, heads, head dim) on the pool's device, head dim contiguous."""
+    if t.device != side.codes.device:
+        raise CqkvError(ERR_ARG, f"{what} is on {t.device}, the page pool on {side.codes.device}")
+    if t.dim() != 3 or t.shape[2] != side.head_dim or (heads is not None and t.shape[1] != heads):
+        raise CqkvError(ERR_ARG, f"{what} {tuple(t.shape)} does not match the pool: (rows, "
+                                 f"{'heads' if heads is None else heads}, {side.head_dim})")
+    if t.numel() and t.stride(2) != 1:
+        raise CqkvError(ERR_ARG, f"{what} needs a contiguous head dim (stride {t.stride()})")
+
+
+def _same_pool(k_side: CacheSide, v_side: CacheSide) -> None:
+    if k_side.batch != v_side.batch or k_side.codes.device != v_side.codes.device:
+        raise CqkvError(ERR_ARG, f"key and value pools differ: {k_side.batch} / {v_side.batch} pages "
+                                 f"on {k_side.codes.device} / {v_side.codes.device}")
+
+
+def _on(device: torch.device):
+    """The pool's device as the current one (the library launches on the current device's streams)."""
+    return torch.cuda.device(device)
+
+
+def paged_append(k_side: CacheSide, v_side: CacheSide, k: torch.Tensor, v: torch.Tensor,
+                 page_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                 positions: torch.Tensor) -> None:
+    """Quantizes packed k / v (total, kv_heads, D) into the pages of a pool: row i of sequence b at
+    position positions[b] + i - cu_seqlens[b]. One launch for both sides."""
+    _same_pool(k_side, v_side)
+    p = _pages(k_side, page_table, cu_seqlens)
+    for t, n in ((k, "k"), (v, "v")):
+        _packed(t, n, k_side, k_side.kv_heads)
+    if k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _DTYPES:
+        raise CqkvError(ERR_ARG, "k and v must have one shape and one dtype (bf16, f16 or f32)")
+    ks, vs = k_side.struct(), v_side.struct()
+    with _on(k.device):
+        _check(lib().cqkv_paged_append(
+            ctypes.byref(ks), ctypes.byref(vs), ctypes.byref(p),
+            _int_array(positions, "positions", p.batch, k.device), _ptr(k), _strides2(k), _ptr(v),
+            _strides2(v), _DTYPES[k.dtype], k.shape[0], _stream(k.device)))
+
+
+def rope_sections(sections) -> list[int]:
+    """The axis of every rotary pair for consecutive sections of pairs, one per axis: (16, 24, 24) is
+    axis 0 for the first 16 pairs, then axis 1, then axis 2."""
+    return [a for a, n in enumerate(sections) for _ in range(n)]
+
+
+def paged_rope_append(k_side: CacheSide, v_side: CacheSide, q: torch.Tensor, k: torch.Tensor,
+                      v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                      rope_positions: torch.Tensor, pair_axis, page_table: torch.Tensor,
+                      cu_seqlens: torch.Tensor, positions: torch.Tensor, kind: int = ROPE_HALVES,
+                      q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_append behind a rotary embedding with several position axes: pair j of row i takes row
+    rope_positions[pair_axis[j], i] of the cos / sin tables (rows, D / 2). rope_positions (axes, total)
+    int32, 1 to 4 axes; pair_axis a sequence of D / 2 axes (rope_sections). Returns the rotated
+    queries (q_out, or a new (total, q_heads, D) tensor; rows outside every sequence are not written)."""
+    _same_pool(k_side, v_side)
+    p = _pages(k_side, page_table, cu_seqlens)
+    _packed(q, "q", k_side)
+    for t, n in ((k, "k"), (v, "v")):
+        _packed(t, n, k_side, k_side.kv_heads)
+    total, hq, d = q.shape
+    dev = q.device
+    if k.shape != v.shape or k.shape[0] != total:
+        raise CqkvError(ERR_ARG, f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} disagree")
+    if len({q.dtype, k.dtype, v.dtype, cos.dtype, sin.dtype}) != 1 or q.dtype not in _DTYPES:
+        raise CqkvError(ERR_ARG, "q, k, v, cos and sin must share one float dtype")
+    if (cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != d // 2 or cos.device != dev
+            or sin.device != dev or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise CqkvError(ERR_ARG, f"cos / sin must be contiguous (rows, {d // 2}) tables on {dev}")
+    if (rope_positions.dim() != 2 or rope_positions.shape[1] != total or rope_positions.device != dev
+            or rope_positions.dtype != torch.int32 or (total > 1 and rope_positions.stride(1) != 1)):
+        raise CqkvError(ERR_ARG, f"rope_positions must be an (axes, {total}) int32 tensor on {dev}")
+    if len(pair_axis) != d // 2 or not all(0 <= a < rope_positions.shape[0] for a in pair_axis):
+        raise CqkvError(ERR_ARG, f"pair_axis must hold {d // 2} axes below {rope_positions.shape[0]}")
+    if q_out is None:
+        q_out = torch.empty((total, hq, d), dtype=q.dtype, device=dev)
+    else:
+        _packed(q_out, "q_out", k_side, hq)
+        if q_out.shape != q.shape or q_out.dtype != q.dtype:
+            raise CqkvError(ERR_ARG, "q_out must match q in shape and dtype")
+    ks, vs = k_side.struct(), v_side.struct()
+    with _on(dev):
+        _check(lib().cqkv_paged_rope_append(
+            ctypes.byref(ks), ctypes.byref(vs), ctypes.byref(p),
+            _int_array(positions, "positions", p.batch, dev), _ptr(q), _strides2(q), _ptr(k),
+            _strides2(k), _ptr(v), _strides2(v), _DTYPES[q.dtype], total, hq, _ptr(cos), _ptr(sin),
+            cos.shape[0], kind, rope_positions.shape[0], _ptr(rope_positions),
+            rope_positions.stride(0), bytes(pair_axis), _ptr(q_out), _strides2(q_out),
+            _stream(dev)))
+    return q_out
+
+
+def paged_dequantize(side: CacheSide, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                     positions: torch.Tensor, total: int, dtype: torch.dtype = torch.float32,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values (total, kv_heads, D) of one side of a pool at the positions that paged_append gives
+    the packed rows. Rows outside every sequence are not written."""
+    p = _pages(side, page_table, cu_seqlens)
+    dev = side.codes.device
+    if out is None:
+        if dtype not in _DTYPES:
+            raise CqkvError(ERR_ARG, f"dtype {dtype} (bf16, f16 or f32)")
+        out = torch.empty((total, side.kv_heads, side.head_dim), dtype=dtype, device=dev)
+    else:
+        _packed(out, "out", side, side.kv_heads)
+        if out.shape[0] != total or out.dtype not in _DTYPES:
+            raise CqkvError(ERR_ARG, f"out {tuple(out.shape)} {out.dtype} does not match {total} rows")
+    s = side.struct()
+    with _on(dev):
+        _check(lib().cqkv_paged_dequantize(
+            ctypes.byref(s), ctypes.byref(p), _int_array(positions, "positions", p.batch, dev), total,
+            _ptr(out), _DTYPES[out.dtype], _strides2(out), _stream(dev)))
+    return out
+
+
+def paged_attention_workspace_bytes(k_side: CacheSide, batch: int, total: int, q_heads: int,
+                                    max_seqlen_q: int, max_seqlen_k: int,
+                                    window_left: int = -1, window_right: int = -1) -> int:
+    """Device bytes that a paged_attention call of these sizes works in (0: none; causal calls have
+    window_right 0)."""
+    s = k_side.struct()
+    return lib().cqkv_paged_attention_workspace_bytes(ctypes.byref(s), batch, total, q_heads,
+                                                      max_seqlen_q, max_seqlen_k, window_left,
+                                                      window_right)
+
+
+def paged_attention(q: torch.Tensor, k_side: CacheSide, v_side: CacheSide, page_table: torch.Tensor,
+                    cu_seqlens_q: torch.Tensor, kv_lens: torch.Tensor, max_seqlen_q: int,
+                    max_seqlen_k: int, softmax_scale: float, causal: bool, window_left: int = -1,
+                    window_right: int = -1, softcap: float = 0.0,
+                    alibi_slopes: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of packed queries (total, q_heads, D), bf16 or f16, over a page pool: sequence b's
+    queries are the last of its first kv_lens[b] positions, whose keys are in the pool already.
+    Single tokens, drafted tokens, chunks of prompts or a mixture. Masks, softcap and alibi_slopes as
+    flash_attn_varlen. Rows outside every sequence are not written."""
+    _same_pool(k_side, v_side)
+    p = _pages(k_side, page_table, cu_seqlens_q)
+    _packed(q, "q", k_side)
+    total, hq, _ = q.shape
+    dev = q.device
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise CqkvError(ERR_ARG, f"q must be bfloat16 or float16, got {q.dtype}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _packed(out, "out", k_side, hq)
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise CqkvError(ERR_ARG, "out must match q in shape and dtype")
+    if causal:
+        window_right = 0
+    al, al_bs = _alibi_arg(alibi_slopes, p.batch, hq)
+    ks, vs = k_side.struct(), v_side.struct()
+    with _on(dev):
+        if workspace is None:
+            workspace = _scratch(lib().cqkv_paged_attention_workspace_bytes(
+                ctypes.byref(ks), p.batch, total, hq, max_seqlen_q, max_seqlen_k, window_left,
+                window_right), dev)
+        _check(lib().cqkv_paged_attention(
+            _ptr(q), _strides2(q), _DTYPES[q.dtype], ctypes.byref(ks), ctypes.byref(vs),
+            ctypes.byref(p), _int_array(kv_lens, "kv_lens", p.batch, dev), total, hq, max_seqlen_q,
+            max_seqlen_k, softmax_scale, window_left, window_right, softcap, al, al_bs, _ptr(out),
+            _strides2(out), _ptr(workspace),
+            0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(dev)))
     return out
 
 

@@ -512,6 +512,87 @@ int cqkv_dequantize_rows(const cqkv_side *side, int32_t batch, int32_t position,
 int cqkv_side_copy(const cqkv_side *dst, const cqkv_side *src, int32_t batch, int32_t tokens,
                    cqkv_stream_t stream);
 
+/* ---- page pools --------------------------------------------------------------------------------
+ * A page pool holds the keys and values of many sequences in pages taken in any order: a key side and
+ * a value side (cqkv_side) whose planes are (page, kv head), page-major - codes / scales hold
+ * n_pages * kv_heads planes - and whose capacity is the page size, a power of two from 32 tokens on.
+ * Formats FP8, MXFP8 and MXFP4, the same on both sides, unrotated; codes and scales 16-byte aligned.
+ * The bytes are those of the dense sides, so cqkv_rows_export and the other side calls read a pool as
+ * a batch of n_pages.
+ *
+ * Tokens are packed: row i of a token tensor belongs to sequence b with cu_seqlens[b] <= i <
+ * cu_seqlens[b + 1]. Rows outside every sequence are neither read nor written. Offsets are clamped
+ * into the `total` rows. Position p of sequence b lies in page table[b * table_stride + p / page size].
+ * Page ids outside [0, n_pages), and positions past the table's max_pages pages, are holes: rows
+ * appended there are dropped, they read back as zeros and their keys are masked. Sequences may share
+ * pages that they only read (a common prefix, the same page twice); two rows of one call appended to
+ * one position of one page, by two sequences that share it, leave a mixture of both.
+ * The arrays are read on the device, in stream order. The calls allocate nothing but the workspace
+ * of cqkv_paged_attention when none is given. */
+typedef struct cqkv_pages {
+    const int32_t *table;      /* device, batch rows of max_pages page ids */
+    int64_t table_stride;      /* elements between the rows (0: one row for every sequence) */
+    const int32_t *cu_seqlens; /* device, batch + 1 prefix sums of the packed rows */
+    int32_t batch;
+    int32_t max_pages;
+    int32_t n_pages;           /* pages of the pool */
+    int32_t reserved;          /* 0 */
+} cqkv_pages;
+
+/* Quantize-and-append into pages: rows k and v (total, kv_heads, D), element strides {token, head} (D
+ * contiguous), dtype CQKV_BF16 / F16 / F32; row i of sequence b lands at position positions[b] + i -
+ * cu_seqlens[b] (device int32, `batch`; a sequence with a negative position is skipped). The codes are
+ * those of cqkv_quant_append. One launch. */
+int cqkv_paged_append(const cqkv_side *k_side, const cqkv_side *v_side, const cqkv_pages *pages,
+                      const int32_t *positions, const void *k, const int64_t k_strides[2],
+                      const void *v, const int64_t v_strides[2], int32_t dtype, int32_t total,
+                      cqkv_stream_t stream);
+
+/* The same behind a rotary embedding with several position axes (time, height, width of image and
+ * video tokens), whose positions are not the cache's: rotary pair j of a head (CQKV_ROPE_HALVES:
+ * elements j, j + D/2; CQKV_ROPE_INTERLEAVED: 2j, 2j + 1) of row i takes the angle in row
+ * rope_positions[axis * rope_stride + i] (device int32; axes 1-4), axis = pair_axis[j] (host, D / 2
+ * entries), of the cos / sin tables (cs_rows, D/2) of `dtype`. q (total, q_heads, D) is rotated into
+ * q_out, k is rotated, rounded to `dtype` as the model's rotated keys are, and appended, v is appended.
+ * A row with a rotary position outside the tables is skipped (q_out, k and v). With one axis and rotary
+ * positions equal to the cache's, this is cqkv_rope_quant_append into pages. One launch. */
+int cqkv_paged_rope_append(const cqkv_side *k_side, const cqkv_side *v_side,
+                           const cqkv_pages *pages, const int32_t *positions, const void *q,
+                           const int64_t q_strides[2], const void *k, const int64_t k_strides[2],
+                           const void *v, const int64_t v_strides[2], int32_t dtype, int32_t total,
+                           int32_t q_heads, const void *cos, const void *sin, int32_t cs_rows,
+                           int32_t rope_kind, int32_t axes, const int32_t *rope_positions,
+                           int64_t rope_stride, const uint8_t *pair_axis, void *q_out,
+                           const int64_t q_out_strides[2], cqkv_stream_t stream);
+
+/* Read-back: row i of out (total, kv_heads, D), strides {token, head}, out_dtype, receives the values
+ * of one side at the position that cqkv_paged_append would give it: scale * value of the code in f32,
+ * rounded to nearest even. */
+int cqkv_paged_dequantize(const cqkv_side *side, const cqkv_pages *pages, const int32_t *positions,
+                          int32_t total, void *out, int32_t out_dtype, const int64_t out_strides[2],
+                          cqkv_stream_t stream);
+
+/* Attention of packed queries over a page pool: single tokens, drafted tokens, chunks of prompts, or a
+ * mixture, as a server batches them. q / out (total, q_heads, D), element strides {token, head}, of
+ * `dtype` (CQKV_BF16 or CQKV_F16). Sequence b attends over its first kv_lens[b] positions (device int32,
+ * clamped to max_kv_len and to the table), its queries bottom-right aligned: they are the last of those
+ * positions, whose keys are in the pool already. window_left / window_right, softcap and alibi_slopes
+ * as cqkv_decode_attention (causal: window_right 0). max_q_len / max_kv_len: the longest sequences
+ * (host), which size the launch; queries past max_q_len are not computed. Rows without a visible key
+ * are zeros. Keys that a query does not see never reach its row, whatever their bytes.
+ * workspace: at least cqkv_paged_attention_workspace_bytes() (0: none needed); NULL = allocated
+ * (stream-ordered) and freed by the call. */
+size_t cqkv_paged_attention_workspace_bytes(const cqkv_side *k_side, int32_t batch, int32_t total,
+                                            int32_t q_heads, int32_t max_q_len, int32_t max_kv_len,
+                                            int32_t window_left, int32_t window_right);
+int cqkv_paged_attention(const void *q, const int64_t q_strides[2], int32_t dtype,
+                         const cqkv_side *k_side, const cqkv_side *v_side, const cqkv_pages *pages,
+                         const int32_t *kv_lens, int32_t total, int32_t q_heads, int32_t max_q_len,
+                         int32_t max_kv_len, float softmax_scale, int32_t window_left,
+                         int32_t window_right, float softcap, const float *alibi_slopes,
+                         int32_t alibi_batch_stride, void *out, const int64_t out_strides[2],
+                         void *workspace, size_t workspace_bytes, cqkv_stream_t stream);
+
 /* TurboQuant tables the kernels use (host): the Lloyd-Max codebook of TurboMse{bits} at head
  * dim D (candle-core/src/accel/turbo.rs:58-129; 2^bits centroids, 2^bits - 1 boundaries) and
  * the Hadamard sign vector of `seed` (turbo.rs:188-203; +1 / -1 per column). */
