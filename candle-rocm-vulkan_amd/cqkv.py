@@ -141,16 +141,15 @@ def lib() -> ctypes.CDLL:
         L.cqkv_dequantize_workspace_bytes.argtypes = [SP, i32, i32, i32]
         L.cqkv_dequantize_workspace_bytes.restype = sz
         L.cqkv_dequantize_rows.argtypes = [SP, i32, i32, i32, i32, P, i32, I64P, P, sz, P]
-        PP = ctypes.POINTER(Pages)
-        i64 = ctypes.c_int64
-        L.cqkv_paged_append.argtypes = [SP, SP, PP, P, P, I64P, P, I64P, i32, i32, P]
-        L.cqkv_paged_rope_append.argtypes = [SP, SP, PP, P, P, I64P, P, I64P, P, I64P, i32, i32, i32,
-                                             P, P, i32, i32, i32, P, i64, P, P, I64P, P]
-        L.cqkv_paged_dequantize.argtypes = [SP, PP, P, i32, P, i32, I64P, P]
-        L.cqkv_paged_attention_workspace_bytes.argtypes = [SP] + [i32] * 7
+        i64 = ctypes.c_int64  # (sides, pages and strides of the page pool calls: packed bytes)
+        L.cqkv_paged_append.argtypes = [P, P, P, P, P, P, P, P, i32, i32, P]
+        L.cqkv_paged_rope_append.argtypes = [P, P, P, P, P, P, P, P, P, P, i32, i32, i32,
+                                             P, P, i32, i32, i32, P, i64, P, P, P, P]
+        L.cqkv_paged_dequantize.argtypes = [P, P, P, i32, P, i32, P, P]
+        L.cqkv_paged_attention_workspace_bytes.argtypes = [P] + [i32] * 7
         L.cqkv_paged_attention_workspace_bytes.restype = sz
-        L.cqkv_paged_attention.argtypes = [P, I64P, i32, SP, SP, PP, P, i32, i32, i32, i32, f32, i32,
-                                           i32, f32, P, i32, P, I64P, P, sz, P]
+        L.cqkv_paged_attention.argtypes = [P, P, i32, P, P, P, P, i32, i32, i32, i32, f32, i32,
+                                           i32, f32, P, i32, P, P, P, sz, P]
         L.cqkv_last_error.restype = ctypes.c_char_p
         L.cqkv_version.restype = ctypes.c_char_p
         _lib = L
@@ -768,53 +767,64 @@ def flash_attn_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 # belongs to the sequence b with cu_seqlens[b] <= i < cu_seqlens[b + 1]. page_table (batch, max_pages)
 # int32; ids outside the pool are holes (appends there are dropped, they read back as zeros, their keys
 # are masked).
-_I64x2 = ctypes.c_int64 * 2
+#
+# The smallest of these calls take 5 us of GPU time, so the arguments are built as in the calls above,
+# and one step further: structures go to the library as packed bytes (0.6 us a side where a ctypes
+# object takes 2) and tensors are compared by device index.
+_PAGES_FIELDS = struct.Struct("QqQ4i")  # the fields of Pages
+_I64x2 = struct.Struct("2q")
+assert _PAGES_FIELDS.size == ctypes.sizeof(Pages)
 
 
-def _strides2(t: torch.Tensor) -> ctypes.Array:
-    return _I64x2(t.stride(0), t.stride(1))
+def _side_bytes(s: CacheSide) -> bytes:
+    return _SIDE_FIELDS.pack(s.fmt, s.is_value, s.head_dim, s.kv_heads, s.capacity, s.rotation, s.bits,
+                             0, s.seed % (1 << 64), s.codes.data_ptr(), s.scales.data_ptr(),
+                             0 if s.qjl is None else s.qjl.data_ptr(),
+                             0 if s.rot is None else s.rot.data_ptr())
 
 
-def _int_array(t: torch.Tensor, what: str, n: int | None, device: torch.device) -> int:
-    if t.device != device or t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 1:
-        raise CqkvError(ERR_ARG, f"{what} must be a contiguous 1-D int32 tensor on {device}")
-    if n is not None and t.numel() != n:
-        raise CqkvError(ERR_ARG, f"{what} has {t.numel()} entries, not {n}")
+def _pool_device(k_side: CacheSide, v_side: CacheSide | None = None) -> int:
+    dev = k_side.codes.get_device()
+    if dev < 0:
+        raise CqkvError(ERR_ARG, f"the page pool must be GPU tensors (got {k_side.codes.device})")
+    if v_side is not None and (v_side.batch != k_side.batch or v_side.codes.get_device() != dev):
+        raise CqkvError(ERR_ARG, f"key and value pools differ: {k_side.batch} / {v_side.batch} pages "
+                                 f"on {k_side.codes.device} / {v_side.codes.device}")
+    return dev
+
+
+def _int_array(t: torch.Tensor, what: str, n: int, dev: int) -> int:
+    if t.get_device() != dev or t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
+        raise CqkvError(ERR_ARG, f"{what} must be a contiguous 1-D int32 tensor on the pool's device")
+    if t.shape[0] != n:
+        raise CqkvError(ERR_ARG, f"{what} has {t.shape[0]} entries, not {n}")
     return t.data_ptr()
 
 
-def _pages(side: CacheSide, page_table: torch.Tensor, cu_seqlens: torch.Tensor) -> Pages:
-    dev = side.codes.device
-    _need_gpu(side.codes, "the page pool")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.device != dev:
-        raise CqkvError(ERR_ARG, f"page_table must be a (batch, max_pages) int32 tensor on {dev}")
+def _pages(side: CacheSide, page_table: torch.Tensor, cu_seqlens: torch.Tensor, dev: int):
+    """The packed cqkv_pages of a call and its batch."""
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.get_device() != dev:
+        raise CqkvError(ERR_ARG, "page_table must be a (batch, max_pages) int32 tensor on the pool's device")
     b, n = page_table.shape
-    if n > 1 and page_table.stride(1) != 1:
+    s0, s1 = page_table.stride()
+    if n > 1 and s1 != 1:
         raise CqkvError(ERR_ARG, "page_table needs contiguous rows")
-    return Pages(page_table.data_ptr(), page_table.stride(0),
-                 _int_array(cu_seqlens, "cu_seqlens", b + 1, dev), b, n, side.batch, 0)
+    return _PAGES_FIELDS.pack(page_table.data_ptr(), s0, _int_array(cu_seqlens, "cu_seqlens", b + 1, dev),
+                              b, n, side.batch, 0), b
 
 
-def _packed(t: torch.Tensor, what: str, side: CacheSide, heads: int | None = None) -> None:
-    """A packed row tensor (total, heads, head dim) on the pool's device, head dim contiguous."""
-    if t.device != side.codes.device:
+def _packed(t: torch.Tensor, what: str, side: CacheSide, dev: int, heads: int | None = None):
+    """Checks a packed row tensor (total, heads, head dim), head dim contiguous, on the pool's device;
+    its packed strides {token, head}."""
+    if t.get_device() != dev:
         raise CqkvError(ERR_ARG, f"{what} is on {t.device}, the page pool on {side.codes.device}")
     if t.dim() != 3 or t.shape[2] != side.head_dim or (heads is not None and t.shape[1] != heads):
         raise CqkvError(ERR_ARG, f"{what} {tuple(t.shape)} does not match the pool: (rows, "
                                  f"{'heads' if heads is None else heads}, {side.head_dim})")
-    if t.numel() and t.stride(2) != 1:
+    s0, s1, s2 = t.stride()
+    if s2 != 1 and t.numel():
         raise CqkvError(ERR_ARG, f"{what} needs a contiguous head dim (stride {t.stride()})")
-
-
-def _same_pool(k_side: CacheSide, v_side: CacheSide) -> None:
-    if k_side.batch != v_side.batch or k_side.codes.device != v_side.codes.device:
-        raise CqkvError(ERR_ARG, f"key and value pools differ: {k_side.batch} / {v_side.batch} pages "
-                                 f"on {k_side.codes.device} / {v_side.codes.device}")
-
-
-def _on(device: torch.device):
-    """The pool's device as the current one (the library launches on the current device's streams)."""
-    return torch.cuda.device(device)
+    return _I64x2.pack(s0, s1)
 
 
 def paged_append(k_side: CacheSide, v_side: CacheSide, k: torch.Tensor, v: torch.Tensor,
@@ -822,24 +832,24 @@ def paged_append(k_side: CacheSide, v_side: CacheSide, k: torch.Tensor, v: torch
                  positions: torch.Tensor) -> None:
     """Quantizes packed k / v (total, kv_heads, D) into the pages of a pool: row i of sequence b at
     position positions[b] + i - cu_seqlens[b]. One launch for both sides."""
-    _same_pool(k_side, v_side)
-    p = _pages(k_side, page_table, cu_seqlens)
-    for t, n in ((k, "k"), (v, "v")):
-        _packed(t, n, k_side, k_side.kv_heads)
+    dev = _pool_device(k_side, v_side)
+    if dev != torch._C._cuda_getDevice():  # the library launches on the current device
+        with torch.cuda.device(dev):
+            return paged_append(k_side, v_side, k, v, page_table, cu_seqlens, positions)
+    p, b = _pages(k_side, page_table, cu_seqlens, dev)
+    ks, vs = (_packed(t, n, k_side, dev, k_side.kv_heads) for t, n in ((k, "k"), (v, "v")))
     if k.shape != v.shape or k.dtype != v.dtype or k.dtype not in _DTYPES:
         raise CqkvError(ERR_ARG, "k and v must have one shape and one dtype (bf16, f16 or f32)")
-    ks, vs = k_side.struct(), v_side.struct()
-    with _on(k.device):
-        _check(lib().cqkv_paged_append(
-            ctypes.byref(ks), ctypes.byref(vs), ctypes.byref(p),
-            _int_array(positions, "positions", p.batch, k.device), _ptr(k), _strides2(k), _ptr(v),
-            _strides2(v), _DTYPES[k.dtype], k.shape[0], _stream(k.device)))
+    _check(lib().cqkv_paged_append(
+        _side_bytes(k_side), _side_bytes(v_side), p, _int_array(positions, "positions", b, dev),
+        k.data_ptr(), ks, v.data_ptr(), vs, _DTYPES[k.dtype], k.shape[0],
+        torch._C._cuda_getCurrentRawStream(dev)))
 
 
-def rope_sections(sections) -> list[int]:
+def rope_sections(sections) -> bytes:
     """The axis of every rotary pair for consecutive sections of pairs, one per axis: (16, 24, 24) is
     axis 0 for the first 16 pairs, then axis 1, then axis 2."""
-    return [a for a, n in enumerate(sections) for _ in range(n)]
+    return bytes(a for a, n in enumerate(sections) for _ in range(n))
 
 
 def paged_rope_append(k_side: CacheSide, v_side: CacheSide, q: torch.Tensor, k: torch.Tensor,
@@ -849,42 +859,47 @@ def paged_rope_append(k_side: CacheSide, v_side: CacheSide, q: torch.Tensor, k: 
                       q_out: torch.Tensor | None = None) -> torch.Tensor:
     """paged_append behind a rotary embedding with several position axes: pair j of row i takes row
     rope_positions[pair_axis[j], i] of the cos / sin tables (rows, D / 2). rope_positions (axes, total)
-    int32, 1 to 4 axes; pair_axis a sequence of D / 2 axes (rope_sections). Returns the rotated
-    queries (q_out, or a new (total, q_heads, D) tensor; rows outside every sequence are not written)."""
-    _same_pool(k_side, v_side)
-    p = _pages(k_side, page_table, cu_seqlens)
-    _packed(q, "q", k_side)
-    for t, n in ((k, "k"), (v, "v")):
-        _packed(t, n, k_side, k_side.kv_heads)
+    int32, 1 to 4 axes; pair_axis the axes of the D / 2 pairs (bytes, as rope_sections makes, or a
+    sequence of ints). Returns the rotated queries (q_out, or a new (total, q_heads, D) tensor; rows
+    outside every sequence are not written)."""
+    dev = _pool_device(k_side, v_side)
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return paged_rope_append(k_side, v_side, q, k, v, cos, sin, rope_positions, pair_axis,
+                                     page_table, cu_seqlens, positions, kind, q_out)
+    p, b = _pages(k_side, page_table, cu_seqlens, dev)
+    qs = _packed(q, "q", k_side, dev)
+    ks, vs = (_packed(t, n, k_side, dev, k_side.kv_heads) for t, n in ((k, "k"), (v, "v")))
     total, hq, d = q.shape
-    dev = q.device
+    dt = q.dtype
     if k.shape != v.shape or k.shape[0] != total:
         raise CqkvError(ERR_ARG, f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} disagree")
-    if len({q.dtype, k.dtype, v.dtype, cos.dtype, sin.dtype}) != 1 or q.dtype not in _DTYPES:
+    if not (dt == k.dtype == v.dtype == cos.dtype == sin.dtype) or dt not in _DTYPES:
         raise CqkvError(ERR_ARG, "q, k, v, cos and sin must share one float dtype")
-    if (cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != d // 2 or cos.device != dev
-            or sin.device != dev or not cos.is_contiguous() or not sin.is_contiguous()):
-        raise CqkvError(ERR_ARG, f"cos / sin must be contiguous (rows, {d // 2}) tables on {dev}")
-    if (rope_positions.dim() != 2 or rope_positions.shape[1] != total or rope_positions.device != dev
-            or rope_positions.dtype != torch.int32 or (total > 1 and rope_positions.stride(1) != 1)):
-        raise CqkvError(ERR_ARG, f"rope_positions must be an (axes, {total}) int32 tensor on {dev}")
-    if len(pair_axis) != d // 2 or not all(0 <= a < rope_positions.shape[0] for a in pair_axis):
-        raise CqkvError(ERR_ARG, f"pair_axis must hold {d // 2} axes below {rope_positions.shape[0]}")
+    if (cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != d // 2 or cos.get_device() != dev
+            or sin.get_device() != dev or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise CqkvError(ERR_ARG, f"cos / sin must be contiguous (rows, {d // 2}) tables on the pool's device")
+    if (rope_positions.dim() != 2 or rope_positions.shape[1] != total
+            or rope_positions.get_device() != dev or rope_positions.dtype != torch.int32
+            or (total > 1 and rope_positions.stride(1) != 1)):
+        raise CqkvError(ERR_ARG, f"rope_positions must be an (axes, {total}) int32 tensor on the pool's device")
+    axes, stride = rope_positions.shape[0], rope_positions.stride(0)
+    try:
+        pair_axis = bytes(pair_axis)
+    except (TypeError, ValueError):
+        raise CqkvError(ERR_ARG, "pair_axis must hold the axes of the rotary pairs") from None
+    if len(pair_axis) != d // 2:
+        raise CqkvError(ERR_ARG, f"pair_axis has {len(pair_axis)} entries, not {d // 2}")
     if q_out is None:
-        q_out = torch.empty((total, hq, d), dtype=q.dtype, device=dev)
-    else:
-        _packed(q_out, "q_out", k_side, hq)
-        if q_out.shape != q.shape or q_out.dtype != q.dtype:
-            raise CqkvError(ERR_ARG, "q_out must match q in shape and dtype")
-    ks, vs = k_side.struct(), v_side.struct()
-    with _on(dev):
-        _check(lib().cqkv_paged_rope_append(
-            ctypes.byref(ks), ctypes.byref(vs), ctypes.byref(p),
-            _int_array(positions, "positions", p.batch, dev), _ptr(q), _strides2(q), _ptr(k),
-            _strides2(k), _ptr(v), _strides2(v), _DTYPES[q.dtype], total, hq, _ptr(cos), _ptr(sin),
-            cos.shape[0], kind, rope_positions.shape[0], _ptr(rope_positions),
-            rope_positions.stride(0), bytes(pair_axis), _ptr(q_out), _strides2(q_out),
-            _stream(dev)))
+        q_out = torch.empty((total, hq, d), dtype=dt, device=q.device)
+    elif q_out.shape != q.shape or q_out.dtype != dt:
+        raise CqkvError(ERR_ARG, "q_out must match q in shape and dtype")
+    _check(lib().cqkv_paged_rope_append(
+        _side_bytes(k_side), _side_bytes(v_side), p, _int_array(positions, "positions", b, dev),
+        q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _DTYPES[dt], total, hq, cos.data_ptr(),
+        sin.data_ptr(), cos.shape[0], kind, axes, rope_positions.data_ptr(), stride, pair_axis,
+        q_out.data_ptr(), _packed(q_out, "q_out", k_side, dev, hq),
+        torch._C._cuda_getCurrentRawStream(dev)))
     return q_out
 
 
@@ -893,21 +908,21 @@ def paged_dequantize(side: CacheSide, page_table: torch.Tensor, cu_seqlens: torc
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """The values (total, kv_heads, D) of one side of a pool at the positions that paged_append gives
     the packed rows. Rows outside every sequence are not written."""
-    p = _pages(side, page_table, cu_seqlens)
-    dev = side.codes.device
+    dev = _pool_device(side)
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return paged_dequantize(side, page_table, cu_seqlens, positions, total, dtype, out)
+    p, b = _pages(side, page_table, cu_seqlens, dev)
     if out is None:
         if dtype not in _DTYPES:
             raise CqkvError(ERR_ARG, f"dtype {dtype} (bf16, f16 or f32)")
-        out = torch.empty((total, side.kv_heads, side.head_dim), dtype=dtype, device=dev)
-    else:
-        _packed(out, "out", side, side.kv_heads)
-        if out.shape[0] != total or out.dtype not in _DTYPES:
-            raise CqkvError(ERR_ARG, f"out {tuple(out.shape)} {out.dtype} does not match {total} rows")
-    s = side.struct()
-    with _on(dev):
-        _check(lib().cqkv_paged_dequantize(
-            ctypes.byref(s), ctypes.byref(p), _int_array(positions, "positions", p.batch, dev), total,
-            _ptr(out), _DTYPES[out.dtype], _strides2(out), _stream(dev)))
+        out = torch.empty((total, side.kv_heads, side.head_dim), dtype=dtype, device=side.codes.device)
+    elif out.dim() != 3 or out.shape[0] != total or out.dtype not in _DTYPES:
+        raise CqkvError(ERR_ARG, f"out {tuple(out.shape)} {out.dtype} does not match {total} rows")
+    _check(lib().cqkv_paged_dequantize(
+        _side_bytes(side), p, _int_array(positions, "positions", b, dev), total, out.data_ptr(),
+        _DTYPES[out.dtype], _packed(out, "out", side, dev, side.kv_heads),
+        torch._C._cuda_getCurrentRawStream(dev)))
     return out
 
 
@@ -916,8 +931,7 @@ def paged_attention_workspace_bytes(k_side: CacheSide, batch: int, total: int, q
                                     window_left: int = -1, window_right: int = -1) -> int:
     """Device bytes that a paged_attention call of these sizes works in (0: none; causal calls have
     window_right 0)."""
-    s = k_side.struct()
-    return lib().cqkv_paged_attention_workspace_bytes(ctypes.byref(s), batch, total, q_heads,
+    return lib().cqkv_paged_attention_workspace_bytes(_side_bytes(k_side), batch, total, q_heads,
                                                       max_seqlen_q, max_seqlen_k, window_left,
                                                       window_right)
 
@@ -932,34 +946,39 @@ def paged_attention(q: torch.Tensor, k_side: CacheSide, v_side: CacheSide, page_
     queries are the last of its first kv_lens[b] positions, whose keys are in the pool already.
     Single tokens, drafted tokens, chunks of prompts or a mixture. Masks, softcap and alibi_slopes as
     flash_attn_varlen. Rows outside every sequence are not written."""
-    _same_pool(k_side, v_side)
-    p = _pages(k_side, page_table, cu_seqlens_q)
-    _packed(q, "q", k_side)
+    dev = _pool_device(k_side, v_side)
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return paged_attention(q, k_side, v_side, page_table, cu_seqlens_q, kv_lens, max_seqlen_q,
+                                   max_seqlen_k, softmax_scale, causal, window_left, window_right,
+                                   softcap, alibi_slopes, out, workspace)
+    p, b = _pages(k_side, page_table, cu_seqlens_q, dev)
+    qs = _packed(q, "q", k_side, dev)
     total, hq, _ = q.shape
-    dev = q.device
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise CqkvError(ERR_ARG, f"q must be bfloat16 or float16, got {q.dtype}")
+    dt = q.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        raise CqkvError(ERR_ARG, f"q must be bfloat16 or float16, got {dt}")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    else:
-        _packed(out, "out", k_side, hq)
-        if out.shape != q.shape or out.dtype != q.dtype:
-            raise CqkvError(ERR_ARG, "out must match q in shape and dtype")
+        out = torch.empty(q.shape, dtype=dt, device=q.device)
+    elif out.shape != q.shape or out.dtype != dt:
+        raise CqkvError(ERR_ARG, "out must match q in shape and dtype")
+    os_ = _packed(out, "out", k_side, dev, hq)
     if causal:
         window_right = 0
-    al, al_bs = _alibi_arg(alibi_slopes, p.batch, hq)
-    ks, vs = k_side.struct(), v_side.struct()
-    with _on(dev):
-        if workspace is None:
-            workspace = _scratch(lib().cqkv_paged_attention_workspace_bytes(
-                ctypes.byref(ks), p.batch, total, hq, max_seqlen_q, max_seqlen_k, window_left,
-                window_right), dev)
-        _check(lib().cqkv_paged_attention(
-            _ptr(q), _strides2(q), _DTYPES[q.dtype], ctypes.byref(ks), ctypes.byref(vs),
-            ctypes.byref(p), _int_array(kv_lens, "kv_lens", p.batch, dev), total, hq, max_seqlen_q,
-            max_seqlen_k, softmax_scale, window_left, window_right, softcap, al, al_bs, _ptr(out),
-            _strides2(out), _ptr(workspace),
-            0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(dev)))
+    al, al_bs = (None, 0) if alibi_slopes is None else _alibi_arg(alibi_slopes, b, hq)
+    ks, L = _side_bytes(k_side), lib()
+    if workspace is None:
+        n = L.cqkv_paged_attention_workspace_bytes(ks, b, total, hq, max_seqlen_q, max_seqlen_k,
+                                                   window_left, window_right)
+        if n:
+            workspace = _scratch(n, q.device)
+    ws, wsb = (None, 0) if workspace is None else (workspace.data_ptr(),
+                                                   workspace.numel() * workspace.element_size())
+    _check(L.cqkv_paged_attention(
+        q.data_ptr(), qs, _DTYPES[dt], ks, _side_bytes(v_side), p,
+        _int_array(kv_lens, "kv_lens", b, dev), total, hq, max_seqlen_q, max_seqlen_k, softmax_scale,
+        window_left, window_right, softcap, al, al_bs, out.data_ptr(), os_, ws, wsb,
+        torch._C._cuda_getCurrentRawStream(dev)))
     return out
 
 

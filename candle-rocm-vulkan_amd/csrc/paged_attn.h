@@ -39,6 +39,9 @@ struct PagedAttnArgs {
     int32_t alibi_bs;
     int32_t splits, tps;     // most key splits of a sequence, 32-key tiles in one
     int32_t col_blocks;      // workgroups along the columns
+    // sequences with more than chunk_from columns per kv head (if the call may have any: chunk_blocks
+    // bounds their column blocks) are the chunk kernel's: splits of chunk_tps of its key tiles
+    int32_t chunk_from, chunk_blocks, chunk_splits, chunk_tps, chunk_bk;
     float *part_o;           // (splits, total * q_heads, D) partial outputs, normalised
     float *part_lse;         // (splits, total * q_heads) log2-sum-exp
 };
@@ -64,6 +67,15 @@ __device__ inline PagedSeq paged_seq(const PagedAttnArgs &a, int b) {
 // most those that the workspace holds (the last one takes what lengths beyond the call's maxima leave).
 __device__ inline int paged_splits(const PagedAttnArgs &a, const PagedSeq &s) {
     return min(max((s.t1 - s.t0 + a.tps - 1) / a.tps, 1), a.splits);
+}
+
+// The same of a sequence that the chunk kernel takes.
+__device__ inline int chunk_splits(const PagedAttnArgs &a, const PagedSeq &s) {
+    const int per = a.chunk_bk / 32, tiles = (s.t1 + per - 1) / per - s.t0 / per;
+    return min(max((tiles + a.chunk_tps - 1) / a.chunk_tps, 1), a.chunk_splits);
+}
+__device__ inline bool chunk_takes(const PagedAttnArgs &a, const PagedSeq &s) {
+    return a.chunk_blocks > 0 && (int64_t)min(s.lq, a.max_q) * a.group > a.chunk_from;
 }
 
 // Head dim held in k-slot 0 of MFMA chunk j by lane group g (the same for K and Q operands).
@@ -480,7 +492,7 @@ __global__ __launch_bounds__((paged_waves<FMT, D, NB>() * 64)) void paged_attn_k
     const PagedSeq sq = paged_seq(a, b);
     const int ncols = min(sq.lq, a.max_q) * a.group, c0 = 16 * NB * cb;
     const int ns = paged_splits(a, sq);
-    if (c0 >= ncols || split >= ns) return;
+    if (c0 >= ncols || split >= ns || chunk_takes(a, sq)) return;
     const int ncb = min(16 * NB, ncols - c0);
 
     PagedCols<NB> col;

@@ -1,5 +1,5 @@
 // Host side of the attention over a page pool (cqkv_paged_attention) and the merge of its key splits.
-#include "paged_attn.h"
+#include "paged_chunk.h"
 
 #include <algorithm>
 
@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a, int
     }
     if (b < 0 || b >= a.pt.batch) return;
     const PagedSeq sq = paged_seq(a, b);
-    const int qi = token - sq.first, ns = paged_splits(a, sq);
+    const int qi = token - sq.first, ns = chunk_takes(a, sq) ? chunk_splits(a, sq) : paged_splits(a, sq);
     if (qi < 0 || qi >= min(sq.lq, a.max_q) || ns < 2) return;
     const bool active = lane < D / 2 / NP;
     const float *lse = a.part_lse + row;
@@ -91,37 +91,56 @@ static int paged_cus() {
     return cache[dev];
 }
 
-// The launch of a call: column blocks of 16 per workgroup, workgroups along the columns, key splits.
+// The launches of a call. Sequences of at most `from` columns per kv head take the decode kernel (nb
+// column blocks of 16 per workgroup), longer ones the chunk kernel.
 struct PagedPlan {
     int nb, col_blocks, splits, tps;
+    int from, waves, chunk_blocks, chunk_splits, chunk_tps, chunk_bk;
     size_t lse, total;  // workspace offsets
 };
 static PagedPlan paged_plan(int32_t format, int32_t d, int32_t batch, int32_t total, int32_t q_heads,
                             int32_t kv_heads, int32_t max_q, int32_t max_kv, int32_t wl, int32_t wr) {
-    PagedPlan p;
-    const int dk = kernel_dim(d);
-    const int64_t cols = (int64_t)max_q * (q_heads / kv_heads);
-    p.nb = cols <= 16 || dk == 256 ? 1 : cols <= 32 ? 2 : 4;
-    p.col_blocks = (int)((cols + 16 * p.nb - 1) / (16 * p.nb));
-    // tiles that a sequence's queries may see: the window's and the chunk's
+    PagedPlan p = {};
+    const int dk = kernel_dim(d), group = q_heads / kv_heads;
+    const int64_t cols = (int64_t)max_q * group;
+    p.from = dk == 256 ? 16 : 64;
+    // the decode kernel's columns (the long sequences of the call are not its)
+    const int64_t few = std::min<int64_t>(cols, p.from / group * group);
+    p.nb = few <= 16 ? 1 : few <= 32 ? 2 : 4;
+    p.col_blocks = (int)((few + 16 * p.nb - 1) / (16 * p.nb));
+    // keys that a sequence's queries may see: the window's and the chunk's
     int64_t keys = max_kv;
     if (wl >= 0) keys = std::min<int64_t>(keys, (int64_t)wl + max_q + std::max(wr, 0));
     const int64_t tiles = (keys + 31) / 32 + 1;
-    const int waves = p.nb == 1 && format != CQKV_FMT_MXFP4 && dk < 256 ? 8 : 4;
+    const int wv = p.nb == 1 && format != CQKV_FMT_MXFP4 && dk < 256 ? 8 : 4;
     // as many workgroups as fill the chip (one of 8 wavefronts per CU, or two of 4), pieces of at
     // least two tiles per wavefront, and of at most 128 tiles, so that sequences of different
     // lengths even out
-    const int64_t wgs = (int64_t)paged_cus() * (8 / waves), planes = (int64_t)batch * kv_heads * p.col_blocks;
+    const int64_t cus = paged_cus();
+    const int64_t wgs = cus * (8 / wv), planes = (int64_t)batch * kv_heads * p.col_blocks;
     int64_t s = std::max<int64_t>((wgs + planes - 1) / std::max<int64_t>(planes, 1), batch > 1 ? (tiles + 127) / 128 : 1);
-    s = std::min(s, std::max<int64_t>(1, tiles / (2 * waves)));
+    s = std::min(s, std::max<int64_t>(1, tiles / (2 * wv)));
     s = std::max<int64_t>(1, std::min<int64_t>(s, 256));
     p.tps = (int)((tiles + s - 1) / s);
     p.splits = (int)((tiles + p.tps - 1) / p.tps);
-    const size_t rows = (size_t)total * q_heads;
-    p.lse = p.total = 0;
-    if (p.splits > 1) {
-        p.lse = ((size_t)p.splits * rows * dk * 4 + 255) & ~(size_t)255;
-        p.total = p.lse + (((size_t)p.splits * rows * 4 + 255) & ~(size_t)255);
+    p.chunk_bk = dk == 256 ? 32 : 64;
+    if (cols > p.from) {
+        // sequences that may have more than `from` columns, and the column blocks they may fill
+        const int64_t all = (int64_t)total * group;
+        p.waves = dk == 256 || cols <= 128 ? 4 : 8;
+        const int64_t nseq = std::min<int64_t>(batch, all / (p.from + 1));
+        p.chunk_blocks = (int)std::min<int64_t>(all / (32 * p.waves) + nseq, 1 << 24);
+        const int64_t ct = (keys + p.chunk_bk - 1) / p.chunk_bk + 1;
+        const int64_t blocks = std::max<int64_t>((int64_t)p.chunk_blocks * kv_heads, 1);
+        int64_t cs = (cus * (8 / p.waves) + blocks - 1) / blocks;
+        cs = std::max<int64_t>(1, std::min<int64_t>({cs, ct / 8, 32}));
+        p.chunk_tps = (int)((ct + cs - 1) / cs);
+        p.chunk_splits = (int)((ct + p.chunk_tps - 1) / p.chunk_tps);
+    }
+    const size_t rows = (size_t)total * q_heads, most = (size_t)std::max(p.splits, p.chunk_splits);
+    if (most > 1) {
+        p.lse = (most * rows * dk * 4 + 255) & ~(size_t)255;
+        p.total = p.lse + ((most * rows * 4 + 255) & ~(size_t)255);
     }
     return p;
 }
@@ -191,6 +210,7 @@ extern "C" int cqkv_paged_attention(const void *q, const int64_t q_strides[2], i
     a.group = q_heads / hkv;
     a.group_m = pf_group_m(a.group);
     a.dim = d;
+    a.o_vec = d % 4 == 0 && (uintptr_t)out % 8 == 0 && a.o_st % 4 == 0 && a.o_sh % 4 == 0;
     a.q_vec = d % 8 == 0 && (uintptr_t)q % 16 == 0 && a.q_st % 8 == 0 && a.q_sh % 8 == 0;
     a.wl = window_left;
     a.wr = window_right;
@@ -203,10 +223,19 @@ extern "C" int cqkv_paged_attention(const void *q, const int64_t q_strides[2], i
     a.splits = p.splits;
     a.tps = p.tps;
     a.col_blocks = p.col_blocks;
-    const int64_t wgs = (int64_t)p.splits * p.col_blocks * pages->batch * hkv;
+    a.chunk_from = p.from;
+    a.chunk_blocks = p.chunk_blocks;
+    a.chunk_splits = p.chunk_splits;
+    a.chunk_tps = p.chunk_tps;
+    a.chunk_bk = p.chunk_bk;
+    // a call whose only sequence is the chunk kernel's has nothing for the decode kernel (a shorter one
+    // than max_q_len says still would: then its columns are counted on the device, so both run)
+    const bool few = p.chunk_blocks == 0 || pages->batch > 1 || total < max_q_len || (int64_t)total * a.group <= p.from;
+    const int64_t wgs = few ? (int64_t)p.splits * p.col_blocks * pages->batch * hkv : 0;
+    const int64_t kgs = (int64_t)p.chunk_splits * p.chunk_blocks * hkv;
     const int64_t cgs = ((int64_t)total * q_heads + 3) / 4;
-    if (wgs > 0x7fffffffll / 256 || cgs > 0x7fffffffll / 256)
-        return fail(CQKV_ERR_ARG, "%s: %lld workgroups exceed one launch", who, (long long)std::max(wgs, cgs));
+    if (wgs > 0x7fffffffll / 512 || cgs > 0x7fffffffll / 256 || kgs > 0x7fffffffll / 512)
+        return fail(CQKV_ERR_ARG, "%s: %lld workgroups exceed one launch", who, (long long)std::max({wgs, cgs, kgs}));
     hipStream_t st = (hipStream_t)stream;
     void *ws = workspace;
     bool owned = false;
@@ -222,12 +251,23 @@ extern "C" int cqkv_paged_attention(const void *q, const int64_t q_strides[2], i
     }
     const int dk = kernel_dim(d);
     const bool f16 = dtype == CQKV_F16;
-    const dim3 grid((unsigned)wgs);
-    if (k_side->format == CQKV_FMT_FP8) paged_attn_launch_5(dk, p.nb, f16, grid, st, a);
-    else if (k_side->format == CQKV_FMT_MXFP8) paged_attn_launch_4(dk, p.nb, f16, grid, st, a);
-    else paged_attn_launch_2(dk, p.nb, f16, grid, st, a);
-    hipError_t e = hipGetLastError();
-    if (e == hipSuccess && p.splits > 1) {
+    const bool logit = a.cap2 > 0.0f || a.alibi;
+    hipError_t e = hipSuccess;
+    if (kgs) {  // the long sequences first: they take longest
+        const dim3 grid((unsigned)kgs);
+        if (k_side->format == CQKV_FMT_FP8) paged_chunk_launch_5(dk, p.waves, f16, logit, grid, st, a);
+        else if (k_side->format == CQKV_FMT_MXFP8) paged_chunk_launch_4(dk, p.waves, f16, logit, grid, st, a);
+        else paged_chunk_launch_2(dk, p.waves, f16, logit, grid, st, a);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess && wgs) {
+        const dim3 grid((unsigned)wgs);
+        if (k_side->format == CQKV_FMT_FP8) paged_attn_launch_5(dk, p.nb, f16, grid, st, a);
+        else if (k_side->format == CQKV_FMT_MXFP8) paged_attn_launch_4(dk, p.nb, f16, grid, st, a);
+        else paged_attn_launch_2(dk, p.nb, f16, grid, st, a);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess && p.total) {
         const dim3 cg((unsigned)cgs);
         if (dk == 64) hipLaunchKernelGGL(paged_combine_kernel<64>, cg, dim3(256), 0, st, a, (int)f16);
         else if (dk == 128) hipLaunchKernelGGL(paged_combine_kernel<128>, cg, dim3(256), 0, st, a, (int)f16);

@@ -1,6 +1,6 @@
 // One format's instantiations of the page pool kernels (compiled once per format with
 // -DCQKV_PAGED_FMT=<format id>, so the formats build in parallel).
-#include "paged_attn.h"
+#include "paged_chunk.h"
 #include "paged_rows.h"
 
 #ifndef CQKV_PAGED_FMT
@@ -25,6 +25,11 @@ void CQKV_CAT(paged_dequant_launch_, CQKV_PAGED_FMT)(int dk, dim3 grid, hipStrea
 void CQKV_CAT(paged_attn_launch_, CQKV_PAGED_FMT)(int dk, int nb, bool f16, dim3 grid, hipStream_t st,
                                                  const PagedAttnArgs &a) {
     launch_paged_attn<CQKV_PAGED_FMT>(dk, nb, f16, grid, st, a);
+}
+
+void CQKV_CAT(paged_chunk_launch_, CQKV_PAGED_FMT)(int dk, int waves, bool f16, bool logit, dim3 grid,
+                                                  hipStream_t st, const PagedAttnArgs &a) {
+    launch_paged_chunk<CQKV_PAGED_FMT>(dk, waves, f16, logit, grid, st, a);
 }
 
 }  // namespace cqkv

@@ -91,23 +91,54 @@ def attention64(q, kvals, vvals, table, cu, kv, scale, wl=-1, wr=0, softcap=0.0,
     return out, mag, wrote
 
 
-def assert_attention(got, want, mag, dtype, fmt4=False):
-    """|got - want| within the roundings of the call: the output to its dtype (half a step of the
-    value, 2^-8 bf16 or 2^-11 f16, of a value that the other errors have moved); the weights as bf16
-    hi + lo parts (2^-16 of the weighted mean of |v|), or one bf16 part for bf16 calls over 4-bit pools
-    (2^-8); f32 scores below 64 in exp2 units with relative error 2^-17 at 256 products of 2^-24 each
-    in chains, i.e. weights to 2^-11 at worst, and 2^-13 for the sums here, where |x| stays below 16."""
+def score_spread(q, kvals, scale):
+    """Largest sum of |q_i k_i| scale of a call's queries and keys (.., .., .., d): the size of a score's
+    terms."""
+    return (q.double().abs().flatten(0, 1) @ kvals.double().abs().amax((0, 1, 2))).max().item() * scale
+
+
+def assert_attention(got, want, mag, dtype, fmt4=False, chunk=False, spread=0.0):
+    """|got - want| within the roundings of the call; mag the weighted mean of |v|.
+
+    The output to its dtype: half a step, 2^-8 (bf16) or 2^-11 (f16) of a value that the other errors
+    have moved. Decode kernel: the weights as bf16 hi + lo parts (2^-16), or one bf16 part for bf16 calls
+    over 4-bit pools (2^-8). Chunk kernel, in the dtype's half step h: the weights (h), the values (h),
+    the keys and the scaled queries (h each, of the terms of a score: these move a weight, and the sum of
+    weights, by 2 x 2 h times at most the sum of |q_i k_i| scale, `spread`, if every term erred its worst
+    way; independent errors stay below a quarter of that, and the largest sum over all keys and queries is
+    taken). f32 sums, exponentials and scores below 32: 2^-13."""
     half = torch.finfo(dtype).eps / 2
-    w = 2.0 ** -13 + (2.0 ** -8 if fmt4 and dtype == torch.bfloat16 else 2.0 ** -16)
+    w = 2.0 ** -13
+    if chunk:
+        w += 2 * half + half * spread
+    else:
+        w += 2.0 ** -8 if fmt4 and dtype == torch.bfloat16 else 2.0 ** -16
     tol = half * want.abs() + (w * (1 + half)) * mag + torch.finfo(dtype).tiny
     err = (got.double().cpu() - want).abs()
     assert bool((err <= tol).all()), f"{(err / tol).max().item():.3f} of the bound, {err.max().item():.3e}"
 
 
+def assert_call(out, q, kvals, vvals, table, cu, kv, scale, dtype, fmt4, **kw):
+    """A whole call against f64, its sequences of few columns (the decode kernel's) and of many (the chunk
+    kernel's) each within their bound; the rows that it does not write hold 77."""
+    want, mag, wrote = attention64(q, kvals, vvals, table, cu, kv, scale, **kw)
+    assert bool((out[~wrote] == 77.0).all())
+    group, d = q.shape[1] // kvals.shape[1], q.shape[2]
+    many = torch.zeros_like(wrote)
+    for a, b in zip(cu.tolist(), cu.tolist()[1:]):
+        many[a:b] = (b - a) * group > (16 if d > 128 else 64)
+    for rows, chunk in ((wrote & ~many, False), (wrote & many, True)):
+        if rows.any():
+            used = [page_rows(kvals, table, b, n) for b, n in enumerate(kv) if n]
+            used = torch.cat([r[ok] for r, ok in used])  # (tokens, heads, d)
+            spread = score_spread(q[rows], used[:, :, None], scale) if chunk else 0.0
+            assert_attention(out[rows], want[rows], mag[rows], dtype, fmt4, chunk, spread)
+
+
 def rope64(x, cos, sin, rope_pos, axes, kind):
     """x (total, heads, d) rotated in f64 (not rounded)."""
     half = x.shape[-1] // 2
-    rows = rope_pos.long()[torch.tensor(axes)]
+    rows = rope_pos.long()[torch.tensor(list(axes))]
     j = torch.arange(half)[:, None]
     c, s = (t.double()[rows, j].t()[:, None] for t in (cos, sin))
     f = x.double()
@@ -121,7 +152,7 @@ def rope64(x, cos, sin, rope_pos, axes, kind):
 def rope32(x, cos, sin, rope_pos, axes, kind):
     """The same with f32 products rounded before the sum, rounded to x's dtype."""
     half = x.shape[-1] // 2
-    rows = rope_pos.long()[torch.tensor(axes)]
+    rows = rope_pos.long()[torch.tensor(list(axes))]
     j = torch.arange(half)[:, None]
     c, s = (t.float()[rows, j].t()[:, None] for t in (cos, sin))
     f = x.float()

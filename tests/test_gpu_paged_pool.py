@@ -351,6 +351,31 @@ ATTN = [
 ]
 
 
+# many (query, head) columns per kv head: the chunk kernel, alone and next to short sequences
+CHUNKS = [
+    (FP8, 128, 8, 2, 64, "bf16", [64], [64]),
+    (FP8, 128, 8, 2, 32, "bf16", [65, 1, 17, 2], [300, 1000, 17, 33]),
+    (FP8, 128, 8, 1, 64, "f16", [33, 100], [700, 100]),
+    (FP8, 128, 32, 2, 32, "bf16", [37], [1500]),
+    (FP8, 64, 4, 4, 32, "bf16", [70, 129, 300], [71, 500, 300]),
+    (FP8, 64, 8, 1, 64, "f16", [9, 40], [900, 41]),
+    (FP8, 256, 4, 2, 64, "bf16", [70, 9, 3], [333, 70, 10]),
+    (FP8, 96, 6, 3, 64, "f16", [90, 4], [200, 100]),
+    (FP8, 80, 2, 1, 32, "bf16", [150], [151]),
+    (FP8, 6, 2, 1, 32, "f16", [100], [133]),
+    (MXFP8, 128, 8, 2, 64, "bf16", [100, 1], [1500, 40]),
+    (MXFP8, 128, 7, 1, 32, "f16", [64, 1], [150, 40]),
+    (MXFP8, 64, 2, 2, 32, "bf16", [290], [300]),
+    (MXFP8, 256, 2, 1, 32, "f16", [50], [130]),
+    (MXFP8, 96, 3, 1, 64, "bf16", [55], [130]),
+    (MXFP4, 128, 8, 2, 64, "bf16", [100, 1], [1500, 40]),
+    (MXFP4, 128, 8, 2, 32, "f16", [40, 1], [150, 40]),
+    (MXFP4, 64, 4, 2, 32, "bf16", [100, 200], [100, 250]),
+    (MXFP4, 256, 2, 1, 256, "bf16", [50], [130]),
+    (MXFP4, 32, 8, 2, 32, "f16", [100], [600]),
+]
+
+
 def run_attention(cq, dev, fmt, d, hq, hkv, page, dtype, new, kv, seed=1, qscale=1.0, extra=0, **kw):
     pages = sum(-(-n // page) for n in kv) + 1
     sides = R.make_pool(cq, dev, fmt, pages, hkv, d, page, seed)
@@ -364,15 +389,17 @@ def run_attention(cq, dev, fmt, d, hq, hkv, page, dtype, new, kv, seed=1, qscale
                        causal, alibi_slopes=None if alibi is None else alibi.to(dev), out=out, **kw)
     vals = [cq.dequantize(s, page).cpu() for s in sides]
     wr = 0 if causal else kw.get("window_right", -1)
-    want, mag, wrote = R.attention64(q, *vals, table.cpu(), cu, kv, R.scale_of(d),
-                                     kw.get("window_left", -1), wr, kw.get("softcap", 0.0), alibi)
-    assert bool((out[~wrote.to(dev)] == 77.0).all())
-    R.assert_attention(out[wrote.to(dev)], want[wrote], mag[wrote], DTYPES[dtype], fmt == MXFP4)
-    return out
+    R.assert_call(out.cpu(), q, *vals, table.cpu(), cu, kv, R.scale_of(d), DTYPES[dtype], fmt == MXFP4,
+                  wl=kw.get("window_left", -1), wr=wr, softcap=kw.get("softcap", 0.0), alibi=alibi)
 
 
 @pytest.mark.parametrize("fmt,d,hq,hkv,page,dtype,new,kv", ATTN)
 def test_attention(cq, dev, fmt, d, hq, hkv, page, dtype, new, kv):
+    run_attention(cq, dev, fmt, d, hq, hkv, page, dtype, new, kv)
+
+
+@pytest.mark.parametrize("fmt,d,hq,hkv,page,dtype,new,kv", CHUNKS)
+def test_attention_chunks(cq, dev, fmt, d, hq, hkv, page, dtype, new, kv):
     run_attention(cq, dev, fmt, d, hq, hkv, page, dtype, new, kv)
 
 
@@ -381,28 +408,34 @@ def test_attention(cq, dev, fmt, d, hq, hkv, page, dtype, new, kv):
     dict(window_left=40), dict(causal=False), dict(causal=False, window_left=10, window_right=5),
     dict(softcap=2.0), dict(window_left=0), dict(window_left=100, softcap=5.0)])
 def test_attention_masks_and_terms(cq, dev, fmt, kw):
-    run_attention(cq, dev, fmt, 128, 8, 2, 32, "bf16", [1, 6, 30], [400, 77, 130], **dict(kw))
+    run_attention(cq, dev, fmt, 128, 8, 2, 32, "bf16", [1, 6, 30, 90], [400, 77, 130, 333], **dict(kw))
+
+
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("kw", [dict(window_left=40), dict(causal=False), dict(softcap=2.0)])
+def test_attention_chunk_masks_other_head_dims(cq, dev, d, kw):
+    run_attention(cq, dev, FP8, d, 4, 2, 32, "f16", [70, 100], [400, 130], **dict(kw))
 
 
 @pytest.mark.parametrize("rows", [1, 2])
 def test_attention_alibi(cq, dev, rows):
     slopes = torch.rand(*((2, 8) if rows == 2 else (8,)), generator=torch.Generator().manual_seed(1)) * 0.05
-    run_attention(cq, dev, FP8, 128, 8, 2, 32, "bf16", [1, 6], [300, 77], alibi=slopes)
+    run_attention(cq, dev, FP8, 128, 8, 2, 32, "bf16", [1, 60], [300, 177], alibi=slopes)
 
 
 @pytest.mark.parametrize("fmt", [FP8, MXFP4])
 def test_attention_peaked(cq, dev, fmt):
     """Large scores: a few keys take all the weight, and the running maximum moves often."""
-    run_attention(cq, dev, fmt, 64, 4, 2, 32, "f16", [1, 6], [300, 77], qscale=4.0)
+    run_attention(cq, dev, fmt, 64, 4, 2, 32, "f16", [1, 6, 80], [300, 77, 300], qscale=4.0)
 
 
 def test_attention_rows_outside_sequences(cq, dev):
-    run_attention(cq, dev, FP8, 64, 4, 2, 32, "bf16", [1, 6, 0, 2], [900, 77, 5, 2], extra=3)
+    run_attention(cq, dev, FP8, 64, 4, 2, 32, "bf16", [1, 6, 0, 2, 80], [900, 77, 5, 2, 400], extra=3)
 
 
 def test_attention_long_split(cq, dev):
     """Keys of one sequence split over the chip, next to short sequences in one split."""
-    run_attention(cq, dev, FP8, 128, 4, 1, 64, "bf16", [1, 1, 2], [5000, 3, 2500])
+    run_attention(cq, dev, FP8, 128, 4, 1, 64, "bf16", [1, 1, 2, 20], [5000, 3, 2500, 4000])
 
 
 def test_attention_shared_pages(cq, dev):
@@ -428,6 +461,14 @@ def test_attention_holes(cq, dev):
     want, mag, _ = R.attention64(q, *[cq.dequantize(s, 32).cpu() for s in sides], table.cpu(), cu, kv, 0.125)
     R.assert_attention(out, want, mag, torch.bfloat16)
     assert bool((out[2:] == 0).all())
+    # the same holes under a chunk
+    cu, n = R.prefix([50, 60], dev), 110
+    q = torch.randn(n, 4, 64, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    out = cq.paged_attention(q.to(dev), *sides, table, cu, R.ints(kv, dev), 60, 128, 0.125, True)
+    vals = [cq.dequantize(s, 32).cpu() for s in sides]
+    want, mag, _ = R.attention64(q, *vals, table.cpu(), cu, kv, 0.125)
+    R.assert_attention(out, want, mag, torch.bfloat16, False, True, R.score_spread(q, vals[0], 0.125))
+    assert bool((out[50:] == 0).all())
 
 
 def test_attention_lengths_are_clamped(cq, dev):
@@ -460,11 +501,11 @@ def poison(cq, dev, side, value, page, table, b, positions):
 
 @pytest.mark.parametrize("fmt", [FP8, MXFP8, MXFP4])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), 3e38, "some"])
-@pytest.mark.parametrize("new", [1, 9, 40])
+@pytest.mark.parametrize("new", [1, 9, 40, 100])
 def test_attention_keys_out_of_sight(cq, dev, fmt, value, new):
     """Rows that a query does not see (behind it, before its window, past the length) may hold NaN,
     infinities or the largest values: they never reach its output."""
-    d, hq, hkv, page, kv, wl = 64, 4, 2, 32, 150, 70
+    d, hq, hkv, page, kv, wl = 64, 4, 2, 32, 180, 70
     sides = R.make_pool(cq, dev, fmt, 6, hkv, d, page, 1)
     table, cu = R.make_table([192], page, 6, dev, 1), R.prefix([new], dev)
     q = torch.randn(new, hq, d, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
@@ -561,8 +602,7 @@ def test_serving_steps(cq, dev, fmt):
         lens = [l + n for l, n in zip(lens, new)]
         out = cq.paged_attention(q, k, v, table, cu, R.ints(lens, dev), max(new), max(lens), 0.125, True)
         vals = [cq.dequantize(s, page).cpu() for s in (k, v)]
-        want, mag, _ = R.attention64(q.cpu(), *vals, table.cpu(), cu, lens, 0.125)
-        R.assert_attention(out, want, mag, torch.bfloat16, fmt == MXFP4)
+        R.assert_call(out.cpu(), q.cpu(), *vals, table.cpu(), cu, lens, 0.125, torch.bfloat16, fmt == MXFP4)
 
 
 def test_captured_step(cq, dev):

@@ -140,4 +140,4 @@ def test_front_end_refuses_cpu_pools(cq):
 
 
 def test_rope_sections(cq):
-    assert cq.rope_sections((2, 1, 3)) == [0, 0, 1, 2, 2, 2]
+    assert list(cq.rope_sections((2, 1, 3))) == [0, 0, 1, 2, 2, 2]
