@@ -18,14 +18,6 @@ struct PageTable {
     int32_t max_pages, n_pages, batch, shift, total;
 };
 
-// First row and length of packed sequence b. Offsets are clamped into [0, total], so inconsistent
-// prefix sums cannot address rows outside the tensors.
-__device__ inline void packed_sequence(const PageTable &p, int b, int &first, int &len) {
-    const scalar_i32 *cu = (const scalar_i32 *)p.cu;
-    first = min(max(cu[b], 0), p.total);
-    len = min(max(cu[b + 1], first), p.total) - first;
-}
-
 // Plane bytes and format of one side of the pool.
 struct PoolSide {
     uint8_t *codes, *scales;

@@ -8,12 +8,13 @@
 // scale of an FP8 row multiplies the score after the product (keys) or the weight before it (values),
 // so quantization is the pool's only rounding of K and V.
 //
-// One workgroup = one (key split, kv head, sequence), its wavefronts taking 32-key tiles in turn; a tile
-// lies in one page, so a page change is a new set of buffer resources in scalar registers. Operand
-// layouts are those of the dense decode kernel: lane (n, g) of v_mfma_f32_16x16x32_bf16 holds column
-// n = a (query, head of the group) pair, keys 8 g .. 8 g + 7 of a tile. NB column blocks of 16 share a
-// tile's loads and its decoded operands, so drafted tokens cost the pool's bytes once. Bound by HBM
-// (FP8, MXFP8) or by the decoding VALU work (MXFP4).
+// A workgroup takes one piece of a (sequence, kv head) plane: a range of its 32-key tiles, its wavefronts
+// taking tiles in turn. A tile lies in one page, so a page change is a new set of buffer resources in
+// scalar registers. Operand layouts are those of the dense decode kernel: lane (n, g) of
+// v_mfma_f32_16x16x32_bf16 holds column n = a (query, head of the group) pair, keys 8 g .. 8 g + 7 of a
+// tile. More than 16 columns (drafted tokens) are blocks of 16 in wavefronts of their own, 2 or 4 on the
+// same tile, whose bytes come from HBM once and from L1 or L2 after that: a wavefront then keeps the
+// registers of one block, and two fit a SIMD. Bound by HBM (FP8, MXFP8) or by the decoding VALU work (MXFP4).
 #pragma once
 
 #include <type_traits>
@@ -37,24 +38,26 @@ struct PagedAttnArgs {
     float scale_log2, cap2;  // cap2: softcap * log2(e), 0: off
     const float *alibi;
     int32_t alibi_bs;
-    int32_t splits, tps;     // most key splits of a sequence, 32-key tiles in one
-    int32_t col_blocks;      // workgroups along the columns
+    int32_t parts;           // pieces of the decode kernel's work (see piece_tiles); 0: one per plane
+    int32_t slot_cols;       // columns of a slot of its partial outputs
     // sequences with more than chunk_from columns per kv head (if the call may have any: chunk_blocks
     // bounds their column blocks) are the chunk kernel's: splits of chunk_tps of its key tiles
     int32_t chunk_from, chunk_blocks, chunk_splits, chunk_tps, chunk_bk;
-    float *part_o;           // (splits, total * q_heads, D) partial outputs, normalised
-    float *part_lse;         // (splits, total * q_heads) log2-sum-exp
+    // Partial outputs, normalised, and their log2-sum-exp: (2 parts, slot_cols) columns of the decode
+    // kernel's pieces, (splits, total * q_heads) rows of the chunk kernel's splits
+    float *part_o, *part_lse, *chunk_o, *chunk_lse;
 };
 
 // A sequence of the call: packed rows, keys, and the 32-key tiles that its queries see.
 struct PagedSeq {
     int first, lq, lk, t0, t1;
 };
-__device__ inline PagedSeq paged_seq(const PagedAttnArgs &a, int b) {
+__device__ inline PagedSeq paged_seq_of(const PagedAttnArgs &a, int cu0, int cu1, int len) {
     PagedSeq s;
-    packed_sequence(a.pt, b, s.first, s.lq);
+    s.first = min(max(cu0, 0), a.pt.total);
+    s.lq = min(max(cu1, s.first), a.pt.total) - s.first;
     const int reach = min(a.max_kv, a.pt.max_pages << a.pt.shift);
-    s.lk = min(max(((const scalar_i32 *)a.kv_lens)[b], 0), reach);
+    s.lk = min(max(len, 0), reach);
     // queries past max_q are not computed: the sequence keeps its alignment, so they are its last ones
     int lo, hi, lo1;
     pf_key_range(0, s.lq, s.lk, a.wl, a.wr, lo, hi);
@@ -63,19 +66,72 @@ __device__ inline PagedSeq paged_seq(const PagedAttnArgs &a, int b) {
     s.t1 = (hi + 31) / 32;
     return s;
 }
-// Splits that the sequence's tiles are cut into: at least one (its rows are written by someone), at
-// most those that the workspace holds (the last one takes what lengths beyond the call's maxima leave).
-__device__ inline int paged_splits(const PagedAttnArgs &a, const PagedSeq &s) {
-    return min(max((s.t1 - s.t0 + a.tps - 1) / a.tps, 1), a.splits);
+__device__ inline PagedSeq paged_seq(const PagedAttnArgs &a, int b) {  // b uniform
+    const scalar_i32 *cu = (const scalar_i32 *)a.pt.cu;
+    return paged_seq_of(a, cu[b], cu[b + 1], ((const scalar_i32 *)a.kv_lens)[b]);
 }
-
-// The same of a sequence that the chunk kernel takes.
+__device__ inline PagedSeq paged_seq_lane(const PagedAttnArgs &a, int b) {  // a sequence per lane
+    if (b >= a.pt.batch) return PagedSeq{0, 0, 0, 0, 0};
+    return paged_seq_of(a, a.pt.cu[b], a.pt.cu[b + 1], a.kv_lens[b]);
+}
+// Splits of a sequence that the chunk kernel takes: at least one (its rows are written by someone), at
+// most those that the workspace holds (the last one takes what lengths beyond the call's maxima leave).
 __device__ inline int chunk_splits(const PagedAttnArgs &a, const PagedSeq &s) {
     const int per = a.chunk_bk / 32, tiles = (s.t1 + per - 1) / per - s.t0 / per;
     return min(max((tiles + a.chunk_tps - 1) / a.chunk_tps, 1), a.chunk_splits);
 }
 __device__ inline bool chunk_takes(const PagedAttnArgs &a, const PagedSeq &s) {
     return a.chunk_blocks > 0 && (int64_t)min(s.lq, a.max_q) * a.group > a.chunk_from;
+}
+
+// ---- pieces ----
+// The launch is made without knowing the lengths, so the workgroups cut the call's planes themselves: into
+// equal pieces of at most U tiles, U = all planes' tiles / parts. Lengths of any mixture then fill the chip
+// (workgroups start as others end), and a captured graph whose lengths grow keeps its balance. At most
+// parts + planes pieces come of it, and at most 2 parts of them belong to planes that are cut (ceil(n / U)
+// <= 2 n / U): those write to their slots, which the combine kernel merges, the others to the output.
+struct SeqWork {
+    int n, pieces;  // tiles of a plane, its pieces (0: nothing for the decode kernel)
+};
+__device__ inline int seq_tiles(const PagedAttnArgs &a, const PagedSeq &s) {  // -1: not the decode kernel's
+    return s.lq > 0 && !chunk_takes(a, s) ? max(s.t1 - s.t0, 0) : -1;
+}
+__device__ inline uint32_t wave_sum_u32(uint32_t v) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) v += (uint32_t)__shfl_xor((int)v, m);
+    return v;
+}
+// Inclusive sum over the lanes of two counts, in the halves of a word.
+__device__ inline uint64_t wave_scan2(uint64_t v, int lane) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)v, m), hi = (uint32_t)__shfl_up((int)(uint32_t)(v >> 32), m);
+        if (lane >= m) v += (uint64_t)hi << 32 | lo;
+    }
+    return v;
+}
+__device__ inline uint64_t readlane64(uint64_t v, int l) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
+}
+// U: at least kPieceTiles tiles, so that a piece's start and merge (about 3 us) stay small beside it.
+constexpr int kPieceTiles = 32;
+__device__ inline uint32_t piece_tiles(const PagedAttnArgs &a, int lane) {
+    uint64_t total = 0;
+    for (int i = 0; i < a.pt.batch; i += 64) {
+        total += wave_sum_u32((uint32_t)max(seq_tiles(a, paged_seq_lane(a, i + lane)), 0));  // (each at most 2^25)
+    }
+    const uint64_t u = (total * (uint32_t)a.kv_heads + (uint32_t)a.parts - 1) / (uint32_t)a.parts;
+    return (uint32_t)min(max(u, (uint64_t)kPieceTiles), (uint64_t)0x40000000u);
+}
+__device__ inline SeqWork seq_work(const PagedAttnArgs &a, const PagedSeq &s, uint32_t u) {
+    const int n = seq_tiles(a, s);
+    return SeqWork{n, n < 0 ? 0 : max((int)(((uint32_t)n + u - 1) / u), 1)};
+}
+// Pieces of a sequence's planes in all, and (high half) those that go to slots.
+__device__ inline uint64_t seq_pieces(const PagedAttnArgs &a, const SeqWork &w) {
+    const uint32_t p = (uint32_t)(w.pieces * a.kv_heads);
+    return (uint64_t)(w.pieces > 1 ? p : 0u) << 32 | p;
 }
 
 // Head dim held in k-slot 0 of MFMA chunk j by lane group g (the same for K and Q operands).
@@ -259,37 +315,30 @@ __device__ inline uint32_t paged_scale_pair(uint32_t p, uint32_t c) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(i16x2, r), i16x2{0, 0}));
 }
 
-// The columns of a lane: keys [lo, hi) of its column, per block of 16.
-template <int NB>
-struct PagedCols {
-    int lo[NB], hi[NB], qpos[NB];
-    float slope2[NB];
+// The column of a lane: its keys [lo, hi).
+struct PagedCol {
+    int lo, hi, qpos;
+    float slope2;
 };
 
 // F16: f16 queries and outputs. The queries enter as bf16 hi + lo parts (exact), the weights too.
-template <int FMT, int D, int NB, bool F16>
+template <int FMT, int D, bool F16>
 __device__ inline void paged_compute(PagedTile<FMT, D> &t, const PagedAttnArgs &a, int key0, int lk,
-                                     bool full, const bf16x8 (*qhi)[D / 32], const bf16x8 (*qlo)[D / 32],
-                                     const PagedCols<NB> &col, int lane, float (&m_run)[NB],
-                                     float (&l_run)[NB], f32x4 (*acc)[D / 16]) {
+                                     bool full, const bf16x8 *qhi, const bf16x8 *qlo, const PagedCol &col,
+                                     int lane, float &m_run, float &l_run, f32x4 *acc) {
     constexpr int NCH = D / 32;
     constexpr bool kFp8 = FMT == CQKV_FMT_FP8;
     constexpr bool LO = F16 || FMT != CQKV_FMT_MXFP4;
     const int g = lane >> 4;
-    f32x4 s0[NB], s1[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) s0[nb] = s1[nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 s0 = {0.f, 0.f, 0.f, 0.f}, s1 = s0;
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
         const bf16x8 k0 = paged_key<FMT, D>(t, 0, j, g), k1 = paged_key<FMT, D>(t, 1, j, g);
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            s0[nb] = mfma16x16x32(k0, qhi[nb][j], s0[nb]);
-            s1[nb] = mfma16x16x32(k1, qhi[nb][j], s1[nb]);
-            if constexpr (F16) {
-                s0[nb] = mfma16x16x32(k0, qlo[nb][j], s0[nb]);
-                s1[nb] = mfma16x16x32(k1, qlo[nb][j], s1[nb]);
-            }
+        s0 = mfma16x16x32(k0, qhi[j], s0);
+        s1 = mfma16x16x32(k1, qhi[j], s1);
+        if constexpr (F16) {
+            s0 = mfma16x16x32(k0, qlo[j], s0);
+            s1 = mfma16x16x32(k1, qlo[j], s1);
         }
     }
     const int kb = key0 + 8 * g;  // the lane's first key
@@ -341,120 +390,117 @@ __device__ inline void paged_compute(PagedTile<FMT, D> &t, const PagedAttnArgs &
         }
         bad = __any(bad);
     }
+    float x[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        float x[8] = {s0[nb].x, s0[nb].y, s0[nb].z, s0[nb].w, s1[nb].x, s1[nb].y, s1[nb].z, s1[nb].w};
+    for (int e = 0; e < 8; ++e) x[e] *= kFp8 ? __uint_as_float(t.ks[e]) * a.scale_log2 : a.scale_log2;
+    if (a.cap2 > 0.0f || a.alibi) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] *= kFp8 ? __uint_as_float(t.ks[e]) * a.scale_log2 : a.scale_log2;
-        if (a.cap2 > 0.0f || a.alibi) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = fa_logit2(x[e], a.cap2, col.slope2[nb], col.qpos[nb] - (kb + e));
-        }
-        uint32_t see = 0xffu;
-        if (!full) {
-            see = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool in = kb + e >= col.lo[nb] && kb + e < col.hi[nb];
-                see |= in ? 1u << e : 0u;
-                if (!in) x[e] = -__builtin_inff();
-            }
-        }
-        float mx = x[0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
-        mx = group16_max(mx);
-        const float m_new = fmaxf(m_run[nb], mx);
-        const bool none = m_new == -__builtin_inff();
-        const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(m_run[nb] - m_new);
-        const float m_sub = none ? 0.0f : m_new;  // scores of -inf then have weight 0, NaN stays NaN
-        float p[8], psum = 0.0f;
+        for (int e = 0; e < 8; ++e) x[e] = fa_logit2(x[e], a.cap2, col.slope2, col.qpos - (kb + e));
+    }
+    uint32_t see = 0xffu;
+    if (!full) {
+        see = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(x[e] - m_sub);
-            psum += p[e];
+            const bool in = kb + e >= col.lo && kb + e < col.hi;
+            see |= in ? 1u << e : 0u;
+            if (!in) x[e] = -__builtin_inff();
         }
-        l_run[nb] = l_run[nb] * alpha + psum;
-        m_run[nb] = m_new;
-        if (__any(alpha != 1.0f)) {
+    }
+    float mx = x[0];
 #pragma unroll
-            for (int i = 0; i < 2 * NCH; ++i) acc[nb][i] *= alpha;
+    for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
+    mx = group16_max(mx);
+    const float m_new = fmaxf(m_run, mx);
+    const bool none = m_new == -__builtin_inff();
+    const float alpha = none ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+    const float m_sub = none ? 0.0f : m_new;  // scores of -inf then have weight 0, NaN stays NaN
+    float p[8], psum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(x[e] - m_sub);
+        psum += p[e];
+    }
+    l_run = l_run * alpha + psum;
+    m_run = m_new;
+    if (__any(alpha != 1.0f)) {
+#pragma unroll
+        for (int i = 0; i < 2 * NCH; ++i) acc[i] *= alpha;
+    }
+    if constexpr (kFp8) {
+        // (a key out of sight keeps weight zero whatever its scale)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] = (see >> e) & 1u ? p[e] * __uint_as_float(t.vs[e]) : 0.0f;
+    }
+    uint32_t hi[4], lo[4];
+    paged_split<LO>(p, hi, lo);
+    // MX: keys out of sight take block byte 0, so that whatever their scale their operand is zero
+    const auto product = [&](const PagedTile<FMT, D> &tv, f32x4 *o, auto masked) {
+        uint32_t keep[4];
+        if constexpr (!kFp8 && masked.value) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                keep[i] = ((see >> (2 * i)) & 1u ? 0xffffu : 0u) | ((see >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
         }
-        if constexpr (kFp8) {
-            // (a key out of sight keeps weight zero whatever its scale)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = (see >> e) & 1u ? p[e] * __uint_as_float(t.vs[e]) : 0.0f;
-        }
-        uint32_t hi[4], lo[4];
-        paged_split<LO>(p, hi, lo);
-        // MX: keys out of sight take block byte 0, so that whatever their scale their operand is zero
-        const auto product = [&](const PagedTile<FMT, D> &tv, f32x4 *o, auto masked) {
-            uint32_t keep[4];
-            if constexpr (!kFp8 && masked.value) {
+        for (int u = 0; u < NCH; ++u) {
+            u32x4 ph, pl;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    keep[i] = ((see >> (2 * i)) & 1u ? 0xffffu : 0u) | ((see >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
-            }
-#pragma unroll
-            for (int u = 0; u < NCH; ++u) {
-                u32x4 ph, pl;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if constexpr (kFp8) {
-                        ph[i] = hi[i];
-                        if constexpr (LO) pl[i] = lo[i];
-                    } else {
-                        uint32_t c = paged_block_pair<D>(tv.vs, i, u);
-                        if constexpr (masked.value) c &= keep[i];
-                        ph[i] = paged_scale_pair(hi[i], c);
-                        if constexpr (LO) pl[i] = paged_scale_pair(lo[i], c);
-                    }
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (kFp8) {
+                    ph[i] = hi[i];
+                    if constexpr (LO) pl[i] = lo[i];
+                } else {
+                    uint32_t c = paged_block_pair<D>(tv.vs, i, u);
+                    if constexpr (masked.value) c &= keep[i];
+                    ph[i] = paged_scale_pair(hi[i], c);
+                    if constexpr (LO) pl[i] = paged_scale_pair(lo[i], c);
                 }
-                const bf16x8 v0 = paged_value<FMT, D>(tv, u, 0), v1 = paged_value<FMT, D>(tv, u, 1);
-                const bf16x8 pb = __builtin_bit_cast(bf16x8, ph);
-                o[2 * u] = mfma16x16x32(v0, pb, o[2 * u]);
-                o[2 * u + 1] = mfma16x16x32(v1, pb, o[2 * u + 1]);
-                if constexpr (LO) {
-                    const bf16x8 pc = __builtin_bit_cast(bf16x8, pl);
-                    o[2 * u] = mfma16x16x32(v0, pc, o[2 * u]);
-                    o[2 * u + 1] = mfma16x16x32(v1, pc, o[2 * u + 1]);
-                }
             }
-        };
-        if (kFp8 ? !bad : full) {
-            product(t, acc[nb], std::false_type{});
-        } else if (!bad) {
-            product(t, acc[nb], std::true_type{});
-        } else {
-            // column by column, each with the codes of the keys it does not see set to zero
+            const bf16x8 v0 = paged_value<FMT, D>(tv, u, 0), v1 = paged_value<FMT, D>(tv, u, 1);
+            const bf16x8 pb = __builtin_bit_cast(bf16x8, ph);
+            o[2 * u] = mfma16x16x32(v0, pb, o[2 * u]);
+            o[2 * u + 1] = mfma16x16x32(v1, pb, o[2 * u + 1]);
+            if constexpr (LO) {
+                const bf16x8 pc = __builtin_bit_cast(bf16x8, pl);
+                o[2 * u] = mfma16x16x32(v0, pc, o[2 * u]);
+                o[2 * u + 1] = mfma16x16x32(v1, pc, o[2 * u + 1]);
+            }
+        }
+    };
+    if (kFp8 ? !bad : full) {
+        product(t, acc, std::false_type{});
+    } else if (!bad) {
+        product(t, acc, std::true_type{});
+    } else {
+        // column by column, each with the codes of the keys it does not see set to zero
 #pragma unroll 1
-            for (int c = 0; c < 16; ++c) {
-                const uint32_t sc = (uint32_t)__shfl((int)see, 16 * g + c);
-                PagedTile<FMT, D> tc = t;
-                uint32_t w0 = 0, w1 = 0;
+        for (int c = 0; c < 16; ++c) {
+            const uint32_t sc = (uint32_t)__shfl((int)see, 16 * g + c);
+            PagedTile<FMT, D> tc = t;
+            uint32_t w0 = 0, w1 = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    w0 |= (sc >> e) & 1u ? 0xffu << (8 * e) : 0u;
-                    w1 |= (sc >> (4 + e)) & 1u ? 0xffu << (8 * e) : 0u;
-                }
-                if constexpr (PagedTile<FMT, D>::B8) {
-#pragma unroll
-                    for (int u = 0; u < NCH; ++u)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            tc.v[u][2 * h] &= w0;
-                            tc.v[u][2 * h + 1] &= w1;
-                        }
-                }
-                f32x4 o[2 * NCH];
-#pragma unroll
-                for (int i = 0; i < 2 * NCH; ++i) o[i] = acc[nb][i];
-                product(tc, o, std::true_type{});
-#pragma unroll
-                for (int i = 0; i < 2 * NCH; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[nb][i][r] = (lane & 15) == c ? o[i][r] : acc[nb][i][r];
+            for (int e = 0; e < 4; ++e) {
+                w0 |= (sc >> e) & 1u ? 0xffu << (8 * e) : 0u;
+                w1 |= (sc >> (4 + e)) & 1u ? 0xffu << (8 * e) : 0u;
             }
+            if constexpr (PagedTile<FMT, D>::B8) {
+#pragma unroll
+                for (int u = 0; u < NCH; ++u)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        tc.v[u][2 * h] &= w0;
+                        tc.v[u][2 * h + 1] &= w1;
+                    }
+            }
+            f32x4 o[2 * NCH];
+#pragma unroll
+            for (int i = 0; i < 2 * NCH; ++i) o[i] = acc[i];
+            product(tc, o, std::true_type{});
+#pragma unroll
+            for (int i = 0; i < 2 * NCH; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][r] = (lane & 15) == c ? o[i][r] : acc[i][r];
         }
     }
 }
@@ -472,195 +518,194 @@ __device__ inline u32x4 paged_q8(const uint16_t *row, int d0, int dim, bool vec)
     return w;
 }
 
-template <int FMT, int D, int NB>
-constexpr int paged_waves() { return FMT != CQKV_FMT_MXFP4 && D < 256 && NB == 1 ? 8 : 4; }
-
-template <int FMT, int D, int NB, bool F16>
-__global__ __launch_bounds__((paged_waves<FMT, D, NB>() * 64)) void paged_attn_kernel(PagedAttnArgs a) {
-    constexpr int NCH = D / 32, WAVES = paged_waves<FMT, D, NB>(), NT = WAVES * 64, kRow = D + 4;
-    __shared__ __attribute__((aligned(16))) float sm_o[WAVES][16][kRow];
+template <int FMT, int D, bool F16>
+__global__ __launch_bounds__(256, (D < 256 ? 2 : 1)) void paged_attn_kernel(PagedAttnArgs a) {
+    constexpr int NCH = D / 32, WAVES = 4;
+    __shared__ __attribute__((aligned(16))) float sm_o[WAVES][16][D + 4];
     __shared__ float sm_m[WAVES][16], sm_l[WAVES][16];
-
-    // planes (sequence, kv head) fastest: with kv heads a multiple of 8 every XCD takes one head of
-    // every sequence, the same mix of lengths everywhere
-    const int planes = a.pt.batch * a.kv_heads;
-    const int rest = (int)blockIdx.x / planes, plane = (int)blockIdx.x % planes;
-    const int split = rest / a.col_blocks, cb = rest % a.col_blocks;
-    const int hk = plane % a.kv_heads, b = plane / a.kv_heads;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 15, g = lane >> 4;
-    const PagedSeq sq = paged_seq(a, b);
-    const int ncols = min(sq.lq, a.max_q) * a.group, c0 = 16 * NB * cb;
-    const int ns = paged_splits(a, sq);
-    if (c0 >= ncols || split >= ns || chunk_takes(a, sq)) return;
-    const int ncb = min(16 * NB, ncols - c0);
 
-    PagedCols<NB> col;
-    bf16x8 qhi[NB][NCH], qlo[NB][NCH];
-    u32x4 qraw[NB][NCH];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        const bool ok = 16 * nb + n < ncb;
-        const int c = c0 + (ok ? 16 * nb + n : 0), qi = pf_div_group(c, a.group, a.group_m);
-        const int head = hk * a.group + (c - qi * a.group);
-        pf_key_range(qi, sq.lq, sq.lk, a.wl, a.wr, col.lo[nb], col.hi[nb]);
-        if (!ok) col.lo[nb] = col.hi[nb] = 0;
-        col.qpos[nb] = qi + sq.lk - sq.lq;
-        col.slope2[nb] = a.alibi && ok ? a.alibi[(int64_t)b * a.alibi_bs + head] * kLog2e : 0.0f;
-        const uint16_t *row = (const uint16_t *)a.q + (int64_t)(sq.first + qi) * a.q_st + (int64_t)head * a.q_sh;
-#pragma unroll
-        for (int j = 0; j < NCH; ++j)
-            qraw[nb][j] = paged_q8(row, paged_qdim<FMT, D>(j, g), ok ? a.dim : 0, a.q_vec);
+    // the piece: sequence, kv head (fastest, so that with 8 kv heads an XCD takes one head of every
+    // sequence: the same mix of lengths everywhere), and its slot
+    int b = -1, rest = 0, slot = -1;
+    uint32_t u = 0;
+    if (a.parts == 0) {
+        b = (int)blockIdx.x / a.kv_heads;
+        rest = (int)blockIdx.x % a.kv_heads;
+    } else {
+        u = piece_tiles(a, lane);
+        uint64_t before = 0;
+        for (int base = 0; base < a.pt.batch; base += 64) {
+            const uint64_t mine = seq_pieces(a, seq_work(a, paged_seq_lane(a, base + lane), u));
+            const uint64_t sum = before + wave_scan2(mine, lane);
+            const uint64_t past = __ballot((uint32_t)sum > blockIdx.x);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                b = base + l;
+                const uint64_t first = readlane64(sum - mine, l);
+                rest = (int)(blockIdx.x - (uint32_t)first);
+                slot = (int)(first >> 32) + rest;
+                break;
+            }
+            before = readlane64(sum, 63);
+        }
+        if (b < 0) return;
     }
-    // keys that every column sees, and the tiles of this split
-    int lo_max, hi_min, unused;
-    pf_key_range(pf_div_group(c0, a.group, a.group_m), sq.lq, sq.lk, a.wl, a.wr, unused, hi_min);
-    pf_key_range(pf_div_group(c0 + ncb - 1, a.group, a.group_m), sq.lq, sq.lk, a.wl, a.wr, lo_max, unused);
-    const int tb = sq.t0 + split * a.tps, te = split == ns - 1 ? sq.t1 : tb + a.tps;
+    const PagedSeq sq = paged_seq(a, b);
+    int hk = rest, tb = sq.t0, te = sq.t1;
+    if (a.parts == 0) {
+        if (seq_tiles(a, sq) < 0) return;
+    } else {
+        const SeqWork w = seq_work(a, sq, u);
+        const int piece = rest / a.kv_heads, len = (int)((uint32_t)w.n / (uint32_t)w.pieces), more = w.n - len * w.pieces;
+        hk = rest - piece * a.kv_heads;
+        tb = sq.t0 + piece * len + min(piece, more);
+        te = tb + len + (piece < more ? 1 : 0);
+        if (w.pieces < 2) slot = -1;
+    }
+
+    // column blocks of 16 in 1, 2 or 4 wavefronts, which take the same tiles
+    const int ncols = min(sq.lq, a.max_q) * a.group;
+    const int cshift = ncols <= 16 ? 0 : ncols <= 32 ? 1 : 2, step = WAVES >> cshift;
+    const int c0 = 16 * (wave & ((1 << cshift) - 1)), ncb = min(16, ncols - c0);
+    int t = tb + (wave >> cshift);
+    if (ncb <= 0) t = te;  // (3 blocks: the fourth wavefront has none)
 
     const scalar_i32 *table = (const scalar_i32 *)a.pt.table + (int64_t)b * a.pt.stride;
     const int tshift = a.pt.shift - 5, tmask = (1 << tshift) - 1;
-    // the page id of a tile; -1 past the split's end
-    const auto page_id = [&](int t) { return t < te ? table[t >> tshift] : -1; };
-    const auto load = [&](PagedTile<FMT, D> &r, int t, int page) {
+    // the page id of a tile; -1 past the end
+    const auto page_id = [&](int i) { return i < te ? table[i >> tshift] : -1; };
+    const auto load = [&](PagedTile<FMT, D> &r, int i, int page) {
         const PageRsrc p = page_rsrc(a, page, hk, (uint32_t)page < (uint32_t)a.pt.n_pages);
-        paged_load<FMT, D>(r, p, 32u * (uint32_t)(t & tmask), lane);
+        paged_load<FMT, D>(r, p, 32u * (uint32_t)(i & tmask), lane);
     };
+    int pa = page_id(t), pc = page_id(t + step);
+
+    PagedCol col;
+    bf16x8 qhi[NCH], qlo[NCH];
+    u32x4 qraw[NCH];
+    {
+        const bool ok = n < ncb;
+        const int c = ok ? c0 + n : 0, qi = pf_div_group(c, a.group, a.group_m);
+        const int head = hk * a.group + (c - qi * a.group);
+        pf_key_range(qi, sq.lq, sq.lk, a.wl, a.wr, col.lo, col.hi);
+        if (!ok) col.lo = col.hi = 0;
+        col.qpos = qi + sq.lk - sq.lq;
+        col.slope2 = a.alibi && ok ? a.alibi[(int64_t)b * a.alibi_bs + head] * kLog2e : 0.0f;
+        const uint16_t *row = (const uint16_t *)a.q + (int64_t)(sq.first + qi) * a.q_st + (int64_t)head * a.q_sh;
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) qraw[j] = paged_q8(row, paged_qdim<FMT, D>(j, g), ok ? a.dim : 0, a.q_vec);
+    }
+    // keys that every column of the wavefront sees
+    int lo_max, hi_min, unused;
+    pf_key_range(pf_div_group(min(c0, ncols - 1), a.group, a.group_m), sq.lq, sq.lk, a.wl, a.wr, unused, hi_min);
+    pf_key_range(pf_div_group(c0 + max(ncb, 1) - 1, a.group, a.group_m), sq.lq, sq.lk, a.wl, a.wr, lo_max, unused);
 
     PagedTile<FMT, D> ta, tc;
-    int t = tb + wave;
-    int pa = page_id(t), pc = page_id(t + WAVES);
     load(ta, t, pa);
     __builtin_amdgcn_sched_barrier(0);
-    load(tc, t + WAVES, pc);
+    load(tc, t + step, pc);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+    for (int j = 0; j < NCH; ++j) {
+        if constexpr (F16) {
+            float x[8];
 #pragma unroll
-        for (int j = 0; j < NCH; ++j) {
-            if constexpr (F16) {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    x[e] = f16_bits_to_f32((qraw[nb][j][e / 2] >> (16 * (e & 1))) & 0xffffu);
-                split_bf16x8(x, qhi[nb][j], qlo[nb][j]);
-            } else {
-                qhi[nb][j] = __builtin_bit_cast(bf16x8, qraw[nb][j]);
-            }
+            for (int e = 0; e < 8; ++e) x[e] = f16_bits_to_f32((qraw[j][e / 2] >> (16 * (e & 1))) & 0xffffu);
+            split_bf16x8(x, qhi[j], qlo[j]);
+        } else {
+            qhi[j] = __builtin_bit_cast(bf16x8, qraw[j]);
         }
-
-    f32x4 acc[NB][2 * NCH];
-    float m_run[NB], l_run[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-        for (int i = 0; i < 2 * NCH; ++i) acc[nb][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        m_run[nb] = -__builtin_inff();
-        l_run[nb] = 0.0f;
     }
-    // a tile in a hole has no keys: its end is before its first key, and its columns see nothing
-    const auto compute = [&](PagedTile<FMT, D> &r, int tt, int page) {
-        const bool hole = (uint32_t)page >= (uint32_t)a.pt.n_pages;
-        if (hole) return;
-        const int key0 = 32 * tt;
+
+    f32x4 acc[2 * NCH];
+#pragma unroll
+    for (int i = 0; i < 2 * NCH; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_run = -__builtin_inff(), l_run = 0.0f;
+    const auto compute = [&](PagedTile<FMT, D> &r, int i, int page) {
+        if ((uint32_t)page >= (uint32_t)a.pt.n_pages) return;  // a hole has no keys
+        const int key0 = 32 * i;
         const bool full = key0 >= lo_max && key0 + 32 <= hi_min;
-        paged_compute<FMT, D, NB, F16>(r, a, key0, sq.lk, full, qhi, qlo, col, lane, m_run, l_run, acc);
+        paged_compute<FMT, D, F16>(r, a, key0, sq.lk, full, qhi, qlo, col, lane, m_run, l_run, acc);
     };
     // register sets alternate; the scheduling barriers keep the loads of one set issued before the
     // next set's, so each wait covers the set about to be used. Page ids are read one step ahead.
-    for (; t < te; t += 2 * WAVES) {
-        const int pa2 = page_id(t + 2 * WAVES), pc2 = page_id(t + 3 * WAVES);
+    for (; t < te; t += 2 * step) {
+        const int pa2 = page_id(t + 2 * step), pc2 = page_id(t + 3 * step);
         compute(ta, t, pa);
         __builtin_amdgcn_sched_barrier(0);
-        load(ta, t + 2 * WAVES, pa2);
+        load(ta, t + 2 * step, pa2);
         __builtin_amdgcn_sched_barrier(0);
-        if (t + WAVES < te) compute(tc, t + WAVES, pc);
+        if (t + step < te) compute(tc, t + step, pc);
         __builtin_amdgcn_sched_barrier(0);
-        load(tc, t + 3 * WAVES, pc2);
+        load(tc, t + 3 * step, pc2);
         __builtin_amdgcn_sched_barrier(0);
         pa = pa2;
         pc = pc2;
     }
 
-    // ---- merge the wavefronts, a block of 16 columns at a time ----
-    const int64_t rows = (int64_t)a.pt.total * a.q_heads;
+    // ---- merge the wavefronts of each column block ----
+    const float l_col = group16_sum(l_run);
+    if (n < ncb) {
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        if (16 * nb >= ncb) break;
-        const int nc = min(16, ncb - 16 * nb);
-        if (nb) __syncthreads();
-        const float l_col = group16_sum(l_run[nb]);
-        if (n < nc) {
+        for (int v = 0; v < NCH; ++v)
 #pragma unroll
-            for (int u = 0; u < NCH; ++u)
-#pragma unroll
-                for (int i = 0; i < 4; i += 2)
-                    *(f32x4 *)&sm_o[wave][n][32 * u + 8 * g + 2 * i] =
-                        f32x4{acc[nb][2 * u][i], acc[nb][2 * u + 1][i], acc[nb][2 * u][i + 1], acc[nb][2 * u + 1][i + 1]};
+            for (int i = 0; i < 4; i += 2)
+                *(f32x4 *)&sm_o[wave][n][32 * v + 8 * g + 2 * i] =
+                    f32x4{acc[2 * v][i], acc[2 * v + 1][i], acc[2 * v][i + 1], acc[2 * v + 1][i + 1]};
+    }
+    if (g == 0) {
+        sm_m[wave][n] = m_run;
+        sm_l[wave][n] = l_col;
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < ncols * (D / 2); idx += WAVES * 64) {
+        const int cc = idx / (D / 2), d = 2 * (idx % (D / 2)), w0 = cc >> 4, c = cc & 15;
+        if (d >= a.dim) continue;  // plane row padding
+        float M = -__builtin_inff();
+        for (int w = w0; w < WAVES; w += 1 << cshift) M = fmaxf(M, sm_m[w][c]);
+        float wsum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+        for (int w = w0; w < WAVES; w += 1 << cshift) {
+            // (a wavefront without a visible key, sum 0, has nothing to add; a NaN sum is kept)
+            const float l = sm_l[w][c], f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(sm_m[w][c] - M);
+            const f32x2 v = *(const f32x2 *)&sm_o[w][c][d];
+            wsum += l * f;
+            o0 += l == 0.0f ? 0.0f : v.x * f;
+            o1 += l == 0.0f ? 0.0f : v.y * f;
         }
-        if (g == 0) {
-            sm_m[wave][n] = m_run[nb];
-            sm_l[wave][n] = l_col;
-        }
-        __syncthreads();
-        for (int idx = threadIdx.x; idx < nc * D; idx += NT) {
-            const int c = idx / D, d = idx % D;
-            if (d >= a.dim) continue;  // plane row padding
-            float M = -__builtin_inff();
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) M = fmaxf(M, sm_m[w][c]);
-            float wsum = 0.0f, osum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) {
-                // (a wavefront without a visible key, sum 0, has nothing to add; a NaN sum is kept)
-                const float f = sm_l[w][c] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(sm_m[w][c] - M);
-                wsum += sm_l[w][c] * f;
-                osum += sm_l[w][c] == 0.0f ? 0.0f : sm_o[w][c][d] * f;
-            }
-            const float o = wsum == 0.0f ? 0.0f : osum / wsum;
-            const float lse = pf_piece_lse(M, wsum);
-            const int cc = c0 + 16 * nb + c, qi = pf_div_group(cc, a.group, a.group_m);
-            const int head = hk * a.group + (cc - qi * a.group);
-            if (ns > 1) {
-                const int64_t row = (int64_t)(sq.first + qi) * a.q_heads + head;
-                a.part_o[(split * rows + row) * D + d] = o;
-                if (d == 0) a.part_lse[split * rows + row] = lse;
-            } else {
-                store_elem(a.out, (int64_t)(sq.first + qi) * a.o_st + (int64_t)head * a.o_sh + d,
-                           F16 ? CQKV_F16 : CQKV_BF16, o);
-            }
+        o0 = wsum == 0.0f ? 0.0f : o0 / wsum;
+        o1 = wsum == 0.0f ? 0.0f : o1 / wsum;
+        if (slot >= 0) {
+            const int64_t at = (int64_t)slot * a.slot_cols + cc;
+            *(f32x2 *)(a.part_o + at * D + d) = f32x2{o0, o1};
+            if (d == 0) a.part_lse[at] = pf_piece_lse(M, wsum);
+        } else {
+            const int qi = pf_div_group(cc, a.group, a.group_m), head = hk * a.group + (cc - qi * a.group);
+            const int64_t at = (int64_t)(sq.first + qi) * a.o_st + (int64_t)head * a.o_sh + d;
+            store_elem(a.out, at, F16 ? CQKV_F16 : CQKV_BF16, o0);
+            if (d + 1 < a.dim) store_elem(a.out, at + 1, F16 ? CQKV_F16 : CQKV_BF16, o1);
         }
     }
 }
 
-// column blocks of 16 that one workgroup takes: 1, 2 or 4 (the rule is the caller's)
-template <int FMT, int D, bool F16>
-inline void launch_paged_attn_d(int nb, dim3 grid, hipStream_t st, const PagedAttnArgs &a) {
-    if (nb == 1 || D == 256)
-        hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 1, F16>), grid, dim3(paged_waves<FMT, D, 1>() * 64), 0, st, a);
-    if constexpr (D < 256) {  // (two blocks at D = 256 do not fit the registers)
-        if (nb == 2)
-            hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 2, F16>), grid, dim3(paged_waves<FMT, D, 2>() * 64), 0, st, a);
-        else if (nb == 4)
-            hipLaunchKernelGGL((paged_attn_kernel<FMT, D, 4, F16>), grid, dim3(paged_waves<FMT, D, 4>() * 64), 0, st, a);
-    }
-}
 template <int FMT>
-inline void launch_paged_attn(int dk, int nb, bool f16, dim3 grid, hipStream_t st, const PagedAttnArgs &a) {
+inline void launch_paged_attn(int dk, bool f16, dim3 grid, hipStream_t st, const PagedAttnArgs &a) {
+#define CQKV_LAUNCH(D)                                                                                        \
+    if (f16) hipLaunchKernelGGL((paged_attn_kernel<FMT, D, true>), grid, dim3(256), 0, st, a);                \
+    else hipLaunchKernelGGL((paged_attn_kernel<FMT, D, false>), grid, dim3(256), 0, st, a)
     if (dk == 64) {
-        if (f16) launch_paged_attn_d<FMT, 64, true>(nb, grid, st, a);
-        else launch_paged_attn_d<FMT, 64, false>(nb, grid, st, a);
+        CQKV_LAUNCH(64);
     } else if (dk == 128) {
-        if (f16) launch_paged_attn_d<FMT, 128, true>(nb, grid, st, a);
-        else launch_paged_attn_d<FMT, 128, false>(nb, grid, st, a);
+        CQKV_LAUNCH(128);
     } else {
-        if (f16) launch_paged_attn_d<FMT, 256, true>(nb, grid, st, a);
-        else launch_paged_attn_d<FMT, 256, false>(nb, grid, st, a);
+        CQKV_LAUNCH(256);
     }
+#undef CQKV_LAUNCH
 }
 
 #define CQKV_PAGED_ATTN_LAUNCHER(F) \
-    void paged_attn_launch_##F(int dk, int nb, bool f16, dim3 grid, hipStream_t st, const PagedAttnArgs &a);
+    void paged_attn_launch_##F(int dk, bool f16, dim3 grid, hipStream_t st, const PagedAttnArgs &a);
 CQKV_PAGED_ATTN_LAUNCHER(2)
 CQKV_PAGED_ATTN_LAUNCHER(4)
 CQKV_PAGED_ATTN_LAUNCHER(5)

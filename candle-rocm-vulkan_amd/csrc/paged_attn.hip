@@ -5,71 +5,136 @@
 
 namespace cqkv {
 
-// Merge of the splits: o = sum_s w_s o_s / sum_s w_s, w_s = 2^(lse_s - max lse). One wavefront per row
-// (packed token, query head); a row outside every sequence, past max_q of its sequence, or of a
-// sequence in one split (written by its only workgroup) is left alone. The row's sequence is the number
-// of prefix sums at or below it, counted 64 at a time.
-template <int D>
-__global__ __launch_bounds__(256) void paged_combine_kernel(PagedAttnArgs a, int out_f16) {
-    constexpr int NP = D == 256 ? 2 : 1;  // element pairs per lane
+// Merge of the pieces: o = sum_s w_s o_s / sum_s w_s, w_s = 2^(lse_s - max lse). A row outside every
+// sequence, past max_q of its sequence, or written whole by its only workgroup is left alone.
+//
+// Bound by latency: the row's sequence has to be found (prefix sums, 64 sequences at a time), then its
+// pieces. D / 4 lanes take a row, so a wavefront has 256 / D heads of a token at once. Few rows (DEEP): a
+// workgroup for them, its 8 wavefronts taking the pieces 8 at a time. Many rows: a wavefront takes `per`
+// such groups of a token, so the sequence is found once for them, two in flight.
+template <int D, bool DEEP>
+__global__ __launch_bounds__(DEEP ? 512 : 256) void paged_combine_kernel(PagedAttnArgs a, int out_f16, int per) {
+    constexpr int LPR = D / 4, RW = 64 / LPR, NG = DEEP ? 1 : 2, NP = DEEP ? 8 : 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = (int64_t)blockIdx.x * 4 + wave, rows = (int64_t)a.pt.total * a.q_heads;
-    if (row >= rows) return;
-    const int token = (int)(row / a.q_heads), head = (int)(row % a.q_heads);
+    const int idx = DEEP ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave;
+    const int groups = (a.q_heads + RW - 1) / RW, runs = (groups + per - 1) / per;
+    const int token = idx / runs, g0 = (idx - token * runs) * per, g1 = min(g0 + per, groups);
+    if (token >= a.pt.total) return;
+    // the sequence, and the slots in front of its
+    const uint32_t u = a.parts ? piece_tiles(a, lane) : 0x40000000u;
     int b = -1;
-    for (int base = 0; base <= a.pt.batch; base += 64) {
-        const bool at = base + lane <= a.pt.batch && min(max(a.pt.cu[base + lane], 0), a.pt.total) <= token;
-        const uint64_t m = __ballot(at);
-        b += __builtin_popcountll(m);
-        if (m != ~0ull) break;
+    uint32_t slots = 0;
+    for (int base = 0; base < a.pt.batch; base += 64) {
+        const PagedSeq ls = paged_seq_lane(a, base + lane);
+        const uint64_t at = __ballot(token >= ls.first && token < ls.first + ls.lq);
+        const uint32_t mine = (uint32_t)(seq_pieces(a, seq_work(a, ls, u)) >> 32);
+        if (at) {
+            const int l = __builtin_ctzll(at);
+            b = base + l;
+            slots += wave_sum_u32(lane < l ? mine : 0u);
+            break;
+        }
+        slots += wave_sum_u32(mine);
     }
-    if (b < 0 || b >= a.pt.batch) return;
+    if (b < 0) return;
     const PagedSeq sq = paged_seq(a, b);
-    const int qi = token - sq.first, ns = chunk_takes(a, sq) ? chunk_splits(a, sq) : paged_splits(a, sq);
-    if (qi < 0 || qi >= min(sq.lq, a.max_q) || ns < 2) return;
-    const bool active = lane < D / 2 / NP;
-    const float *lse = a.part_lse + row;
-    float M = -__builtin_inff();
-    for (int s = lane; s < ns; s += 64) M = fmaxf(M, lse[s * rows]);
-    M = wave_max(M);
-    float wsum = 0.0f, acc[2 * NP] = {};
-    const float *po = a.part_o + row * D + 2 * (active ? lane : 0);
-    const int64_t step = rows * D;
-    for (int s0 = 0; s0 < ns; s0 += 64) {
-        const int nn = min(ns - s0, 64);
-        const float e = lane < nn ? lse[(s0 + lane) * rows] : -__builtin_inff();
-        const float w = e == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(e - M);
-        for (int s1 = 0; s1 < nn; s1 += 8) {
-            f32x2 v[8][NP];
+    const int qi = token - sq.first;
+    if (qi >= min(sq.lq, a.max_q)) return;
+    const bool chunk = chunk_takes(a, sq);
+    const int np = chunk ? chunk_splits(a, sq) : seq_work(a, sq, u).pieces;
+    if (np < 2) return;
+    const float *pl = chunk ? a.chunk_lse : a.part_lse, *po = chunk ? a.chunk_o : a.part_o;
+    const int64_t step = chunk ? (int64_t)a.pt.total * a.q_heads : (int64_t)a.kv_heads * a.slot_cols;
+    const int d0 = 4 * (lane % LPR);
+    for (int gg = g0; gg < g1; gg += NG) {
+        float M[NG], wsum[NG];
+        f32x4 acc[NG];
+        int head[NG];
+        int64_t at[NG];  // piece s: row at + s * step of the partials
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < NG; ++i) {
+            M[i] = -__builtin_inff();
+            wsum[i] = 0.0f;
+            acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            head[i] = min(min(gg + i, g1 - 1) * RW + lane / LPR, a.q_heads - 1);
+            const int hk = pf_div_group(head[i], a.group, a.group_m);
+            at[i] = chunk ? (int64_t)token * a.q_heads + head[i]
+                          : (int64_t)(slots + (uint32_t)hk) * a.slot_cols + qi * a.group + (head[i] - hk * a.group);
+        }
+        for (int s0 = DEEP ? NP * wave : 0; s0 < np; s0 += DEEP ? 8 * NP : NP) {
+            float e[NG][NP];
+            f32x4 v[NG][NP];
 #pragma unroll
-                for (int p = 0; p < NP; ++p)
-                    v[i][p] = *(const f32x2 *)(po + (s0 + min(s1 + i, nn - 1)) * step + 128 * p);
+            for (int i = 0; i < NG; ++i)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (s1 + i >= nn) break;
-                const float ws = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), s1 + i));
-                if (ws == 0.0f) continue;
-                wsum += ws;
+                for (int j = 0; j < NP; ++j) {
+                    const int64_t row = at[i] + min(s0 + j, np - 1) * step;
+                    e[i][j] = pl[row];
+                    v[i][j] = *(const f32x4 *)(po + row * D + d0);
+                }
 #pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    acc[2 * p] += ws * v[i][p].x;
-                    acc[2 * p + 1] += ws * v[i][p].y;
+            for (int i = 0; i < NG; ++i) {
+                float mx = M[i];
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    if (s0 + j >= np) e[i][j] = -__builtin_inff();
+                    mx = fmaxf(mx, e[i][j]);
+                }
+                const float f = M[i] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(M[i] - mx);
+                acc[i] *= f;
+                wsum[i] *= f;
+                M[i] = mx;
+#pragma unroll
+                for (int j = 0; j < NP; ++j) {
+                    // (a piece without a visible key, or too small to count, adds nothing; NaN is kept)
+                    const float w = e[i][j] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(e[i][j] - mx);
+                    wsum[i] += w;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[i][c] += w == 0.0f ? 0.0f : w * v[i][j][c];
                 }
             }
         }
-    }
-    if (!active) return;
-    const int64_t at = (int64_t)token * a.o_st + (int64_t)head * a.o_sh;
+        if constexpr (DEEP) {
+            __shared__ f32x4 sm_acc[8][64];
+            __shared__ float sm_m[8][64], sm_w[8][64];
+            sm_acc[wave][lane] = acc[0];
+            sm_m[wave][lane] = M[0];
+            sm_w[wave][lane] = wsum[0];
+            __syncthreads();
+            if (wave) return;
+            for (int w = 1; w < 8; ++w) M[0] = fmaxf(M[0], sm_m[w][lane]);
+            acc[0] = f32x4{0.f, 0.f, 0.f, 0.f};
+            wsum[0] = 0.0f;
 #pragma unroll
-    for (int p = 0; p < NP; ++p)
+            for (int w = 0; w < 8; ++w) {
+                const float l = sm_w[w][lane], f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(sm_m[w][lane] - M[0]);
+                const f32x4 v = sm_acc[w][lane];
+                wsum[0] += l * f;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int j = 128 * p + 2 * lane + e;
-            const float o = wsum == 0.0f ? 0.0f : acc[2 * p + e] / wsum;
-            if (j < a.dim) store_elem(a.out, at + j, out_f16 ? CQKV_F16 : CQKV_BF16, o);
+                for (int c = 0; c < 4; ++c) acc[0][c] += f == 0.0f ? 0.0f : v[c] * f;
+            }
         }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            if (gg + i >= g1 || (gg + i) * RW + lane / LPR >= a.q_heads) continue;
+            const int64_t out = (int64_t)token * a.o_st + (int64_t)head[i] * a.o_sh + d0;
+            f32x4 o;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[c] = wsum[i] == 0.0f ? 0.0f : acc[i][c] / wsum[i];
+            if (a.o_vec) {
+                if (d0 < a.dim) {
+                    u32x2 w;
+                    if (out_f16) w = u32x2{pack_f16x2(o.x, o.y), pack_f16x2(o.z, o.w)};
+                    else w = u32x2{pack_bf16x2(o.x, o.y), pack_bf16x2(o.z, o.w)};
+                    *(u32x2 *)((uint16_t *)a.out + out) = w;
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (d0 + c < a.dim) store_elem(a.out, out + c, out_f16 ? CQKV_F16 : CQKV_BF16, o[c]);
+            }
+        }
+    }
 }
 
 static int paged_cus() {
@@ -91,57 +156,71 @@ static int paged_cus() {
     return cache[dev];
 }
 
-// The launches of a call. Sequences of at most `from` columns per kv head take the decode kernel (nb
-// column blocks of 16 per workgroup), longer ones the chunk kernel.
+// The launches of a call. Sequences of at most `from` columns per kv head take the decode kernel, longer
+// ones the chunk kernel.
 struct PagedPlan {
-    int nb, col_blocks, splits, tps;
-    int from, waves, chunk_blocks, chunk_splits, chunk_tps, chunk_bk;
-    size_t lse, total;  // workspace offsets
+    int parts, slot_cols;
+    int from, chunk_blocks, chunk_splits, chunk_tps, chunk_bk;
+    size_t part_lse, chunk_o, chunk_lse, total;  // workspace offsets and size
 };
-static PagedPlan paged_plan(int32_t format, int32_t d, int32_t batch, int32_t total, int32_t q_heads,
-                            int32_t kv_heads, int32_t max_q, int32_t max_kv, int32_t wl, int32_t wr) {
+static PagedPlan paged_plan(int32_t d, int32_t batch, int32_t total, int32_t q_heads, int32_t kv_heads, int32_t max_q,
+                            int32_t max_kv, int32_t wl, int32_t wr) {
     PagedPlan p = {};
     const int dk = kernel_dim(d), group = q_heads / kv_heads;
-    const int64_t cols = (int64_t)max_q * group;
-    p.from = dk == 256 ? 16 : 64;
-    // the decode kernel's columns (the long sequences of the call are not its)
-    const int64_t few = std::min<int64_t>(cols, p.from / group * group);
-    p.nb = few <= 16 ? 1 : few <= 32 ? 2 : 4;
-    p.col_blocks = (int)((few + 16 * p.nb - 1) / (16 * p.nb));
+    const int64_t cols = (int64_t)max_q * group, cus = paged_cus();
     // keys that a sequence's queries may see: the window's and the chunk's
     int64_t keys = max_kv;
     if (wl >= 0) keys = std::min<int64_t>(keys, (int64_t)wl + max_q + std::max(wr, 0));
-    const int64_t tiles = (keys + 31) / 32 + 1;
-    const int wv = p.nb == 1 && format != CQKV_FMT_MXFP4 && dk < 256 ? 8 : 4;
-    // as many workgroups as fill the chip (one of 8 wavefronts per CU, or two of 4), pieces of at
-    // least two tiles per wavefront, and of at most 128 tiles, so that sequences of different
-    // lengths even out
-    const int64_t cus = paged_cus();
-    const int64_t wgs = cus * (8 / wv), planes = (int64_t)batch * kv_heads * p.col_blocks;
-    int64_t s = std::max<int64_t>((wgs + planes - 1) / std::max<int64_t>(planes, 1), batch > 1 ? (tiles + 127) / 128 : 1);
-    s = std::min(s, std::max<int64_t>(1, tiles / (2 * wv)));
-    s = std::max<int64_t>(1, std::min<int64_t>(s, 256));
-    p.tps = (int)((tiles + s - 1) / s);
-    p.splits = (int)((tiles + p.tps - 1) / p.tps);
+    p.from = 64;
+    const bool many = cols > p.from;
+    if (many && batch == 1) p.from = 0;  // the one sequence: no launch for short ones
+    const int64_t rows = (int64_t)total * q_heads;
+    size_t at = 0;
+    const auto take = [&](int64_t floats) {
+        const size_t o = at;
+        at += ((size_t)floats * 4 + 255) & ~(size_t)255;
+        return o;
+    };
+    p.slot_cols = (int)((std::min<int64_t>(cols, p.from) + 15) / 16 * 16);
+    if (keys > 32 * kPieceTiles && p.from) {
+        // one round of the chip's workgroups where the planes leave half of them to cut with (4 sequences of
+        // up to 128K keys, MXFP4, 64 / 8 heads: 88 us; three rounds: 132), else three, so that the last one is
+        // short (64 sequences of up to 8K keys, FP8, 32 / 8 heads: 129 us; one round of a plane each: 155)
+        const int64_t slots = cus * (dk < 256 ? 2 : 1), planes = (int64_t)batch * kv_heads;
+        p.parts = (int)(2 * planes <= slots ? slots - planes : 3 * slots);
+        // slots: at most 2 parts, and one more than the parts for every plane
+        const int64_t cut = std::min<int64_t>(2 * p.parts, p.parts + planes);
+        take(cut * p.slot_cols * dk);
+        p.part_lse = take(cut * p.slot_cols);
+    }
     p.chunk_bk = dk == 256 ? 32 : 64;
-    if (cols > p.from) {
-        // sequences that may have more than `from` columns, and the column blocks they may fill
+    if (many) {
+        // column blocks: those that sequences of more than `from` columns may fill (the launch), and those
+        // that they fill if max_q is the longest one's length (the splits)
         const int64_t all = (int64_t)total * group;
-        p.waves = dk == 256 || cols <= 128 ? 4 : 8;
-        const int64_t nseq = std::min<int64_t>(batch, all / (p.from + 1));
-        p.chunk_blocks = (int)std::min<int64_t>(all / (32 * p.waves) + nseq, 1 << 24);
-        const int64_t ct = (keys + p.chunk_bk - 1) / p.chunk_bk + 1;
-        const int64_t blocks = std::max<int64_t>((int64_t)p.chunk_blocks * kv_heads, 1);
-        int64_t cs = (cus * (8 / p.waves) + blocks - 1) / blocks;
-        cs = std::max<int64_t>(1, std::min<int64_t>({cs, ct / 8, 32}));
-        p.chunk_tps = (int)((ct + cs - 1) / cs);
+        const int nc = 32 * chunk_waves(dk);
+        p.chunk_blocks = (int)std::min<int64_t>(all / nc + std::min<int64_t>(batch, all / (p.from + 1)), 1 << 24);
+        const int64_t rest = std::max<int64_t>(all - cols, 0);
+        const int64_t blocks = ((cols + nc - 1) / nc + (rest + nc - 1) / nc * (rest > (int64_t)p.from * (batch - 1))) * kv_heads;
+        // as many splits as end soonest: rounds of the chip over the length of a split
+        const int64_t ct = (keys + p.chunk_bk - 1) / p.chunk_bk + 1, slots = cus;
+        int best = 1;
+        double cost = 1e30;
+        for (int cs = 1; cs <= 16 && (cs == 1 || ct / cs >= 8); ++cs) {
+            const double c = (double)((blocks * cs + slots - 1) / slots) * ((double)ct / cs + 4.0);
+            if (c < cost * 0.97) {
+                best = cs;
+                cost = c;
+            }
+        }
+        p.chunk_tps = (int)((ct + best - 1) / best);
         p.chunk_splits = (int)((ct + p.chunk_tps - 1) / p.chunk_tps);
+        if (p.chunk_splits > 1) {
+            p.chunk_o = take(p.chunk_splits * rows * dk);
+            p.chunk_lse = take(p.chunk_splits * rows);
+        }
     }
-    const size_t rows = (size_t)total * q_heads, most = (size_t)std::max(p.splits, p.chunk_splits);
-    if (most > 1) {
-        p.lse = (most * rows * dk * 4 + 255) & ~(size_t)255;
-        p.total = p.lse + ((most * rows * 4 + 255) & ~(size_t)255);
-    }
+    p.total = at;
     return p;
 }
 
@@ -157,8 +236,8 @@ extern "C" size_t cqkv_paged_attention_workspace_bytes(const cqkv_side *k_side, 
     if (check_side(k_side, "cqkv_paged_attention_workspace_bytes") != CQKV_OK || batch <= 0 ||
         total <= 0 || q_heads <= 0 || q_heads % k_side->kv_heads || max_q_len <= 0 || max_kv_len <= 0)
         return 0;
-    return paged_plan(k_side->format, k_side->head_dim, batch, total, q_heads, k_side->kv_heads, max_q_len,
-                      max_kv_len, window_left, window_right)
+    return paged_plan(k_side->head_dim, batch, total, q_heads, k_side->kv_heads, max_q_len, max_kv_len,
+                      window_left, window_right)
         .total;
 }
 
@@ -218,23 +297,23 @@ extern "C" int cqkv_paged_attention(const void *q, const int64_t q_strides[2], i
     a.cap2 = softcap * kLog2e;
     a.alibi = alibi_slopes;
     a.alibi_bs = alibi_batch_stride;
-    const PagedPlan p = paged_plan(k_side->format, d, pages->batch, total, q_heads, hkv, max_q_len, max_kv_len, window_left,
+    const PagedPlan p = paged_plan(d, pages->batch, total, q_heads, hkv, max_q_len, max_kv_len, window_left,
                                    window_right);
-    a.splits = p.splits;
-    a.tps = p.tps;
-    a.col_blocks = p.col_blocks;
+    a.parts = p.parts;
+    a.slot_cols = p.slot_cols;
     a.chunk_from = p.from;
     a.chunk_blocks = p.chunk_blocks;
     a.chunk_splits = p.chunk_splits;
     a.chunk_tps = p.chunk_tps;
     a.chunk_bk = p.chunk_bk;
-    // a call whose only sequence is the chunk kernel's has nothing for the decode kernel (a shorter one
-    // than max_q_len says still would: then its columns are counted on the device, so both run)
-    const bool few = p.chunk_blocks == 0 || pages->batch > 1 || total < max_q_len || (int64_t)total * a.group <= p.from;
-    const int64_t wgs = few ? (int64_t)p.splits * p.col_blocks * pages->batch * hkv : 0;
+    const int64_t wgs = p.from ? p.parts + (int64_t)pages->batch * hkv : 0;
     const int64_t kgs = (int64_t)p.chunk_splits * p.chunk_blocks * hkv;
-    const int64_t cgs = ((int64_t)total * q_heads + 3) / 4;
-    if (wgs > 0x7fffffffll / 512 || cgs > 0x7fffffffll / 256 || kgs > 0x7fffffffll / 512)
+    // the merge: head groups of a token, few with a workgroup each, many in runs that make 4096 wavefronts
+    const int64_t groups = (q_heads * kernel_dim(d) + 255) / 256;
+    const bool deep = total * groups <= 512;
+    const int per = deep ? 1 : (int)std::clamp<int64_t>(total * groups / 4096, 1, 8);
+    const int64_t runs = total * ((groups + per - 1) / per), cgs = deep ? runs : (runs + 3) / 4;
+    if (wgs > 0x7fffffffll / 512 || cgs > 0x7fffffffll / 256 || runs > 0x7fffffffll - 4 || kgs > 0x7fffffffll / 512)
         return fail(CQKV_ERR_ARG, "%s: %lld workgroups exceed one launch", who, (long long)std::max({wgs, cgs, kgs}));
     hipStream_t st = (hipStream_t)stream;
     void *ws = workspace;
@@ -247,7 +326,9 @@ extern "C" int cqkv_paged_attention(const void *q, const int64_t q_strides[2], i
             owned = true;
         }
         a.part_o = (float *)ws;
-        a.part_lse = (float *)((char *)ws + p.lse);
+        a.part_lse = (float *)((char *)ws + p.part_lse);
+        a.chunk_o = (float *)((char *)ws + p.chunk_o);
+        a.chunk_lse = (float *)((char *)ws + p.chunk_lse);
     }
     const int dk = kernel_dim(d);
     const bool f16 = dtype == CQKV_F16;
@@ -255,23 +336,30 @@ extern "C" int cqkv_paged_attention(const void *q, const int64_t q_strides[2], i
     hipError_t e = hipSuccess;
     if (kgs) {  // the long sequences first: they take longest
         const dim3 grid((unsigned)kgs);
-        if (k_side->format == CQKV_FMT_FP8) paged_chunk_launch_5(dk, p.waves, f16, logit, grid, st, a);
-        else if (k_side->format == CQKV_FMT_MXFP8) paged_chunk_launch_4(dk, p.waves, f16, logit, grid, st, a);
-        else paged_chunk_launch_2(dk, p.waves, f16, logit, grid, st, a);
+        if (k_side->format == CQKV_FMT_FP8) paged_chunk_launch_5(dk, f16, logit, grid, st, a);
+        else if (k_side->format == CQKV_FMT_MXFP8) paged_chunk_launch_4(dk, f16, logit, grid, st, a);
+        else paged_chunk_launch_2(dk, f16, logit, grid, st, a);
         e = hipGetLastError();
     }
     if (e == hipSuccess && wgs) {
         const dim3 grid((unsigned)wgs);
-        if (k_side->format == CQKV_FMT_FP8) paged_attn_launch_5(dk, p.nb, f16, grid, st, a);
-        else if (k_side->format == CQKV_FMT_MXFP8) paged_attn_launch_4(dk, p.nb, f16, grid, st, a);
-        else paged_attn_launch_2(dk, p.nb, f16, grid, st, a);
+        if (k_side->format == CQKV_FMT_FP8) paged_attn_launch_5(dk, f16, grid, st, a);
+        else if (k_side->format == CQKV_FMT_MXFP8) paged_attn_launch_4(dk, f16, grid, st, a);
+        else paged_attn_launch_2(dk, f16, grid, st, a);
         e = hipGetLastError();
     }
     if (e == hipSuccess && p.total) {
-        const dim3 cg((unsigned)cgs);
-        if (dk == 64) hipLaunchKernelGGL(paged_combine_kernel<64>, cg, dim3(256), 0, st, a, (int)f16);
-        else if (dk == 128) hipLaunchKernelGGL(paged_combine_kernel<128>, cg, dim3(256), 0, st, a, (int)f16);
-        else hipLaunchKernelGGL(paged_combine_kernel<256>, cg, dim3(256), 0, st, a, (int)f16);
+#define CQKV_COMBINE(D)                                                                                           \
+    if (deep) hipLaunchKernelGGL((paged_combine_kernel<D, true>), dim3(cgs), dim3(512), 0, st, a, (int)f16, per); \
+    else hipLaunchKernelGGL((paged_combine_kernel<D, false>), dim3(cgs), dim3(256), 0, st, a, (int)f16, per)
+        if (dk == 64) {
+            CQKV_COMBINE(64);
+        } else if (dk == 128) {
+            CQKV_COMBINE(128);
+        } else {
+            CQKV_COMBINE(256);
+        }
+#undef CQKV_COMBINE
         e = hipGetLastError();
     }
     if (owned) {

@@ -749,9 +749,9 @@ __global__ __launch_bounds__(W * 64, 1) void paged_chunk_kernel(PagedAttnArgs a)
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (ns > 1) {  // this split's normalised rows and their log2-sum-exp
         const int64_t rows = (int64_t)a.pt.total * a.q_heads, row = split * rows + token * a.q_heads + head;
-        if (h == 0) a.part_lse[row] = pf_piece_lse(st.m_run, l);
+        if (h == 0) a.chunk_lse[row] = pf_piece_lse(st.m_run, l);
         if (l == 0.0f) return;  // no weight: the merge does not read the row
-        float *po = a.part_o + row * D + 4 * h;
+        float *po = a.chunk_o + row * D + 4 * h;
 #pragma unroll
         for (int md = 0; md < G::MD; ++md)
 #pragma unroll
@@ -778,36 +778,29 @@ __global__ __launch_bounds__(W * 64, 1) void paged_chunk_kernel(PagedAttnArgs a)
         }
 }
 
-template <int FMT, int D, bool F16, bool LOGIT>
-inline void launch_paged_chunk_l(int waves, dim3 grid, hipStream_t st, const PagedAttnArgs &a) {
-    if constexpr (D < 256) {
-        if (waves == 8) {
-            hipLaunchKernelGGL((paged_chunk_kernel<FMT, D, 8, F16, LOGIT>), grid, dim3(512), 0, st, a);
-            return;
-        }
-    }
-    hipLaunchKernelGGL((paged_chunk_kernel<FMT, D, 4, F16, LOGIT>), grid, dim3(256), 0, st, a);
-}
+// Wavefronts of 32 columns in a workgroup: 8 fill a CU, so a tile is converted once there (32 / 8 heads, a
+// chunk of 512 against 16K keys, FP8, D = 128: 159 us; 4 wavefronts, two workgroups a CU: 251); at D = 256
+// the registers allow 4.
+constexpr int chunk_waves(int d) { return d < 256 ? 8 : 4; }
+
 template <int FMT, int D>
-inline void launch_paged_chunk_d(int waves, bool f16, bool logit, dim3 grid, hipStream_t st, const PagedAttnArgs &a) {
-    if (f16) {
-        if (logit) launch_paged_chunk_l<FMT, D, true, true>(waves, grid, st, a);
-        else launch_paged_chunk_l<FMT, D, true, false>(waves, grid, st, a);
-    } else {
-        if (logit) launch_paged_chunk_l<FMT, D, false, true>(waves, grid, st, a);
-        else launch_paged_chunk_l<FMT, D, false, false>(waves, grid, st, a);
-    }
+inline void launch_paged_chunk_d(bool f16, bool logit, dim3 grid, hipStream_t st, const PagedAttnArgs &a) {
+    constexpr int W = chunk_waves(D);
+    const dim3 block(64 * W);
+    if (f16 && logit) hipLaunchKernelGGL((paged_chunk_kernel<FMT, D, W, true, true>), grid, block, 0, st, a);
+    else if (f16) hipLaunchKernelGGL((paged_chunk_kernel<FMT, D, W, true, false>), grid, block, 0, st, a);
+    else if (logit) hipLaunchKernelGGL((paged_chunk_kernel<FMT, D, W, false, true>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((paged_chunk_kernel<FMT, D, W, false, false>), grid, block, 0, st, a);
 }
 template <int FMT>
-inline void launch_paged_chunk(int dk, int waves, bool f16, bool logit, dim3 grid, hipStream_t st, const PagedAttnArgs &a) {
-    if (dk == 64) launch_paged_chunk_d<FMT, 64>(waves, f16, logit, grid, st, a);
-    else if (dk == 128) launch_paged_chunk_d<FMT, 128>(waves, f16, logit, grid, st, a);
-    else launch_paged_chunk_d<FMT, 256>(waves, f16, logit, grid, st, a);
+inline void launch_paged_chunk(int dk, bool f16, bool logit, dim3 grid, hipStream_t st, const PagedAttnArgs &a) {
+    if (dk == 64) launch_paged_chunk_d<FMT, 64>(f16, logit, grid, st, a);
+    else if (dk == 128) launch_paged_chunk_d<FMT, 128>(f16, logit, grid, st, a);
+    else launch_paged_chunk_d<FMT, 256>(f16, logit, grid, st, a);
 }
 
-#define CQKV_PAGED_CHUNK_LAUNCHER(F)                                                                   \
-    void paged_chunk_launch_##F(int dk, int waves, bool f16, bool logit, dim3 grid, hipStream_t st, \
-                                const PagedAttnArgs &a);
+#define CQKV_PAGED_CHUNK_LAUNCHER(F) \
+    void paged_chunk_launch_##F(int dk, bool f16, bool logit, dim3 grid, hipStream_t st, const PagedAttnArgs &a);
 CQKV_PAGED_CHUNK_LAUNCHER(2)
 CQKV_PAGED_CHUNK_LAUNCHER(4)
 CQKV_PAGED_CHUNK_LAUNCHER(5)
