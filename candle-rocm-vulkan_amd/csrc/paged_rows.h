@@ -13,6 +13,8 @@
 // LDS and no barrier. Bound by HBM; single tokens by the latency of the chain sequence -> page -> row.
 #pragma once
 
+#include <type_traits>
+
 #include "paged.h"
 
 namespace cqkv {
@@ -29,12 +31,13 @@ struct PagedRowsArgs {
     const int32_t *rope_pos;   // (axes, total)
     int64_t rope_stride;
     uint32_t axis[8];          // 2 bits per rotary pair: its axis
-    uint32_t mixed;            // bit c: the pairs of table chunk c (8 pairs) have different axes
+    uint32_t mixed;            // the pairs of some 8 neighbours have different axes
     int32_t cs_rows, axes;
     int32_t dim, dtype, kv_heads, q_heads;
     int32_t vec;               // rows, tables and strides are whole 16-byte pieces (16-bit dtypes)
     int32_t q_units, k_units, v_units;  // head groups of a tile's q, k and v
-    int32_t units;             // their sum
+    int32_t per;               // groups of k and q that a wavefront takes (append)
+    int32_t units;             // wavefronts of a tile
     // read-back
     void *out;
     int64_t out_st, out_sh;
@@ -113,47 +116,78 @@ __device__ inline void load_any8(const void *x, int64_t row, int j0, int dim, in
 // Axis of rotary pair j.
 __device__ inline int pair_axis(const PagedRowsArgs &a, int j) { return (a.axis[j >> 4] >> (2 * (j & 15))) & 3; }
 
-// cos and sin of the 8 pairs (halves: pairs j0 .. j0 + 7 of the elements, modulo dim / 2) or 4 pairs
-// (interleaved, each twice) of elements e0 .. e0 + 7 of token row i.
-template <int ROPE>
-__device__ inline void load_angles(const PagedRowsArgs &a, const int (&row)[4], int e0, bool live,
-                                   float (&c)[8], float (&s)[8]) {
-    const int half = a.dim / 2;
-    if constexpr (ROPE == CQKV_ROPE_HALVES) {
-        const int j0 = e0 >= half ? e0 - half : e0;
-        if (a.vec && !((a.mixed >> (j0 >> 3)) & 1)) {
-            const int ax = pair_axis(a, min(j0, half - 1));
-            const int r = ax == 0 ? row[0] : ax == 1 ? row[1] : ax == 2 ? row[2] : row[3];
-            u32x4 cw = {0u, 0u, 0u, 0u}, sw = cw;
-            if (live) {
-                cw = *(const u32x4 *)((const uint16_t *)a.cos + (int64_t)r * half + j0);
-                sw = *(const u32x4 *)((const uint16_t *)a.sin + (int64_t)r * half + j0);
-            }
-            raw_to_f32x8(cw, a.dtype == CQKV_BF16, c);
-            raw_to_f32x8(sw, a.dtype == CQKV_BF16, s);
-            return;
+__device__ inline int axis_row(const int (&row)[4], int ax) {
+    return ax == 0 ? row[0] : ax == 1 ? row[1] : ax == 2 ? row[2] : row[3];
+}
+
+// cos and sin of the pairs of elements e0 .. e0 + 7, as they are in the tables (16-bit): halves the 8 pairs
+// e0 .. modulo dim / 2, interleaved the 4 pairs e0 / 2 .. in two words.
+template <int ROPE, bool MIXED>
+__device__ inline void load_angles(const PagedRowsArgs &a, const int (&row)[4], int e0, u32x4 &c, u32x4 &s) {
+    const int half = a.dim / 2, j0 = ROPE == CQKV_ROPE_INTERLEAVED ? e0 >> 1 : e0 >= half ? e0 - half : e0;
+    const uint16_t *ct = (const uint16_t *)a.cos + j0, *st = (const uint16_t *)a.sin + j0;
+    if constexpr (!MIXED) {  // one axis for them
+        const int64_t at = (int64_t)axis_row(row, pair_axis(a, j0)) * half;
+        if constexpr (ROPE == CQKV_ROPE_INTERLEAVED) {
+            const u32x2 cw = *(const u32x2 *)(ct + at), sw = *(const u32x2 *)(st + at);
+            c = u32x4{cw.x, cw.y, 0u, 0u};
+            s = u32x4{sw.x, sw.y, 0u, 0u};
+        } else {
+            c = *(const u32x4 *)(ct + at);
+            s = *(const u32x4 *)(st + at);
         }
+        return;
     }
+    c = s = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < (ROPE == CQKV_ROPE_INTERLEAVED ? 4 : 8); ++i) {
+        const int64_t at = (int64_t)axis_row(row, pair_axis(a, j0 + i)) * half + i;
+        c[i / 2] |= (uint32_t)ct[at] << (16 * (i & 1));
+        s[i / 2] |= (uint32_t)st[at] << (16 * (i & 1));
+    }
+}
+// The same of any dtype, as f32 (interleaved: element e's pair is entry e & ~1).
+template <int ROPE>
+__device__ inline void load_angles_any(const PagedRowsArgs &a, const int (&row)[4], int e0, bool live,
+                                       float (&c)[8], float (&s)[8]) {
+    const int half = a.dim / 2;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const int j = ROPE == CQKV_ROPE_HALVES ? (e0 + e >= half ? e0 + e - half : e0 + e) : (e0 + e) >> 1;
         c[e] = s[e] = 0.0f;
-        if (!live || e0 + e >= a.dim) continue;
-        if (ROPE == CQKV_ROPE_INTERLEAVED && (e & 1)) {
-            c[e] = c[e - 1];
-            s[e] = s[e - 1];
-            continue;
-        }
-        const int ax = pair_axis(a, j);
-        const int r = ax == 0 ? row[0] : ax == 1 ? row[1] : ax == 2 ? row[2] : row[3];
-        c[e] = load_elem(a.cos, (int64_t)r * half + j, a.dtype);
-        s[e] = load_elem(a.sin, (int64_t)r * half + j, a.dtype);
+        if (!live || e0 + e >= a.dim || (ROPE == CQKV_ROPE_INTERLEAVED && (e & 1))) continue;
+        const int64_t at = (int64_t)axis_row(row, pair_axis(a, j)) * half + j;
+        c[e] = load_elem(a.cos, at, a.dtype);
+        s[e] = load_elem(a.sin, at, a.dtype);
     }
+}
+
+// The 8 elements dim / 2 away from the lane's, which another lane of the row holds.
+template <int LPR>
+__device__ inline u32x4 partner8(const u32x4 &w, const PagedRowsArgs &a, int e0, int lane) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int v = (int)w[i];
+        if (a.dim != 8 * LPR) {
+            r[i] = (uint32_t)__shfl(v, lane + (e0 >= a.dim / 2 ? -(a.dim / 16) : a.dim / 16));
+        } else if constexpr (LPR == 8) {  // lane ^ 7, then ^ 3
+            const int m = __builtin_amdgcn_mov_dpp(v, 0x141, 0xF, 0xF, true);
+            r[i] = (uint32_t)__builtin_amdgcn_mov_dpp(m, 0x1B, 0xF, 0xF, true);
+        } else if constexpr (LPR == 16) {  // row_ror:8
+            r[i] = (uint32_t)__builtin_amdgcn_mov_dpp(v, 0x128, 0xF, 0xF, true);
+        } else {
+            const auto x = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+            r[i] = lane & 16 ? x[0] : x[1];
+        }
+    }
+    return r;
 }
 
 // x rotated: y0 = x0 c - x1 s, y1 = x0 s + x1 c of every pair, products rounded before the sum as in
 // the dense rotary kernels, then rounded to the dtype (a rotated row is a row of the dtype; the codes
-// of the pages are those of that row). px: the partners of a halves pair.
+// of the pages are those of that row). px: the partners of a halves pair; interleaved: entries 0, 2, 4, 6
+// of c and s are the pairs'.
 template <int ROPE>
 __device__ inline void rotate8(float (&x)[8], const float (&px)[8], const float (&c)[8],
                                const float (&s)[8], int e0, int half, int dtype) {
@@ -176,9 +210,10 @@ __device__ inline void rotate8(float (&x)[8], const float (&px)[8], const float 
 }
 
 // Codes of a lane's 8 elements (8-bit: two words; 4-bit: one) and the scale: FP8 the row's f32, MX the
-// block's E8M0 byte (a block is the 8-element chunks of four lanes).
-template <int FMT, int LPR>
-__device__ inline void encode8(const float (&x)[8], u32x2 &cw, float &tok, uint32_t &blk) {
+// block's E8M0 byte (a block is the 8-element chunks of four lanes). False where the lane needs the
+// software encoders (an element that is not finite, an FP8 row of extreme magnitude) and ANY is not set.
+template <int FMT, int LPR, bool ANY>
+__device__ inline bool encode8(const float (&x)[8], u32x2 &cw, float &tok, uint32_t &blk) {
     float m = 0.0f, chk = 0.0f;  // chk: NaN iff an element is not finite
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -190,7 +225,9 @@ __device__ inline void encode8(const float (&x)[8], u32x2 &cw, float &tok, uint3
         const float amax = row_max_lanes<LPR>(m);
         const float sc = amax > 0.0f ? amax / 448.0f : 1.0f, rc = 1.0f / sc;
         tok = sc;
-        if (chk == chk && amax >= kFp8FastRowMin && amax <= 3.0e38f) {
+        // (a row of zeros too: s = 1, every quotient the zero of its element)
+        const bool plain = chk == chk && amax <= 3.0e38f && (amax >= kFp8FastRowMin || amax == 0.0f);
+        if (!ANY || plain) {
 #pragma unroll
             for (int w = 0; w < 2; ++w)
                 cw[w] = fp8_row_codes_fast(x[4 * w], x[4 * w + 1], sc, rc) |
@@ -201,13 +238,14 @@ __device__ inline void encode8(const float (&x)[8], u32x2 &cw, float &tok, uint3
                 cw[w] = fp8_row_codes(x[4 * w], x[4 * w + 1], sc, rc) |
                         (fp8_row_codes(x[4 * w + 2], x[4 * w + 3], sc, rc) << 16);
         }
+        return ANY || plain;
     } else {
         constexpr bool kFp4 = FMT == CQKV_FMT_MXFP4;
         blk = mx_scale_code(quad_max(m), kFp4 ? 2 : 8);
-        if (blk == 0) return;
+        if (blk == 0) return true;
         const float scale = e8m0_to_f32(blk), rs = 1.0f / scale;  // a power of two: exact
         // a NaN in any of the block's lanes is encoded by the software encoders, of the whole chunk
-        if (chk == chk) {
+        if (!ANY || chk == chk) {
             if constexpr (kFp4) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -227,6 +265,7 @@ __device__ inline void encode8(const float (&x)[8], u32x2 &cw, float &tok, uint3
                 cw[kFp4 ? 0 : e / 4] |= c << (kFp4 ? 4 * e : 8 * (e % 4));
             }
         }
+        return ANY || chk == chk;
     }
 }
 
@@ -292,141 +331,11 @@ __device__ inline bool angle_rows(const PagedRowsArgs &a, int64_t i, int (&r)[4]
     return in;
 }
 
-template <int FMT, int D, int ROPE, bool VEC>
-__device__ inline void rows_unit(const PagedRowsArgs &a, const TileAt &t, int unit, int lane) {
-    constexpr int LPR = D / 8, RPW = 64 / LPR;
-    constexpr bool kB8 = FMT != CQKV_FMT_MXFP4;
-    const int c = lane % LPR, e0 = 8 * c, half = a.dim / 2;
-    // the unit's kind: keys, values or queries (uniform)
-    const int kind = unit < a.k_units ? 0 : unit < a.k_units + a.v_units ? 1 : 2;
-    const int group = kind == 0 ? unit : kind == 1 ? unit - a.k_units : unit - a.k_units - a.v_units;
-    const int h = group * RPW + lane / LPR;
-    const bool mine = h < (kind == 2 ? a.q_heads : a.kv_heads);
-    int page = 0;
-    if (kind != 2 && !page_of(a.pt, t.b, t.tile, page)) return;
-    const void *x = kind == 0 ? a.kx : kind == 1 ? a.vx : a.q;
-    const int64_t st = kind == 0 ? a.k_st : kind == 1 ? a.v_st : a.q_st;
-    const int64_t sh = kind == 0 ? a.k_sh : kind == 1 ? a.v_sh : a.q_sh;
-    const int s_lo = max(t.pos - 8 * t.tile, 0), s_hi = min(t.pos + t.len - 8 * t.tile, 8);
-    const int64_t row0 = t.first + (int64_t)8 * t.tile - t.pos;  // packed row of slot 0
-    const bool rope = ROPE != 0 && kind != 1;
-
-    // the slots written: those of the call's rows, without the ones whose angles lie outside the tables
-    uint32_t live = 0;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-        if (s < s_lo || s >= s_hi) continue;
-        int r[4];
-        if (ROPE != 0 && !angle_rows(a, row0 + s, r)) continue;
-        live |= 1u << s;
-    }
-    if (!live) return;
-
-    const PoolSide &side = kind == 0 ? a.k : a.v;
-    const int64_t plane = (int64_t)page * a.kv_heads + (mine ? h : 0);
-    const int in_page = t.tile & ((1 << (a.pt.shift - 3)) - 1);  // the tile's place in its page
-    uint8_t *codes = side.codes + plane * side.codes_plane;
-    uint8_t *scales = side.scales + plane * side.scales_plane;
-
-    // slot s's elements: the queries go out, keys and values are encoded
-    const auto finish = [&](int s, const float (&y)[8]) {
-        u32x2 w = {0u, 0u};
-        if (kind == 2) {
-            if (!mine) return w;
-            const int64_t o = (row0 + s) * a.o_st + h * a.o_sh + e0;
-            if (VEC && e0 < a.dim) {
-                u32x4 ow;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    ow[i] = a.dtype == CQKV_BF16 ? pack_bf16x2(y[2 * i], y[2 * i + 1]) : pack_f16x2(y[2 * i], y[2 * i + 1]);
-                *(u32x4 *)((uint16_t *)a.q_out + o) = ow;
-            } else if (!VEC) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (e0 + e < a.dim) store_elem(a.q_out, o + e, a.dtype, y[e]);
-            }
-            return w;
-        }
-        float tok = 0.0f;
-        uint32_t blk = 0;
-        encode8<FMT, LPR>(y, w, tok, blk);
-        if (!mine) return w;
-        const int row = 8 * in_page + s;
-        if constexpr (FMT == CQKV_FMT_FP8) {
-            if (c == 0) ((float *)scales)[row] = tok;
-        } else if ((c & 3) == 0) {
-            scales[row * (D / 32) + c / 4] = (uint8_t)blk;
-        }
-        if (kind == 0) {
-            if constexpr (kB8) *(u32x2 *)(codes + (int64_t)row * D + e0) = w;
-            else *(uint32_t *)(codes + (int64_t)row * (D / 2) + 4 * c) = w.x;
-        }
-        return w;
-    };
-
-    u32x2 cw[8];
-    if constexpr (VEC) {
-        u32x4 raw[8], par[8];
-        const uint16_t *base = (const uint16_t *)x + h * sh + e0;
-        const bool in = mine && e0 < a.dim;
-        const int pofs = e0 >= half ? -half : half;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            raw[s] = par[s] = u32x4{0u, 0u, 0u, 0u};
-            if (in && ((live >> s) & 1)) {
-                raw[s] = *(const u32x4 *)(base + (row0 + s) * st);
-                if (ROPE == CQKV_ROPE_HALVES && rope) par[s] = *(const u32x4 *)(base + (row0 + s) * st + pofs);
-            }
-        }
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            cw[s] = u32x2{0u, 0u};
-            if (!((live >> s) & 1)) continue;
-            float y[8];
-            raw_to_f32x8(raw[s], a.dtype == CQKV_BF16, y);
-            if (ROPE != 0 && rope) {
-                int r[4];
-                float px[8], cc[8], ss[8];
-                angle_rows(a, row0 + s, r);
-                raw_to_f32x8(par[s], a.dtype == CQKV_BF16, px);
-                load_angles<ROPE>(a, r, e0, in, cc, ss);
-                rotate8<ROPE>(y, px, cc, ss, e0, half, a.dtype);
-            }
-            cw[s] = finish(s, y);
-        }
-    } else {
-#pragma unroll
-        for (int s = 0; s < 8; ++s) cw[s] = u32x2{0u, 0u};
-#pragma unroll 1
-        for (int s = 0; s < 8; ++s) {
-            if (!((live >> s) & 1)) continue;
-            const int64_t row = (row0 + s) * st + h * sh;
-            float y[8];
-            load_any8(x, row, e0, mine ? a.dim : 0, a.dtype, y);
-            if (ROPE != 0 && rope) {
-                int r[4];
-                float px[8] = {}, cc[8], ss[8];
-                angle_rows(a, row0 + s, r);
-                if (ROPE == CQKV_ROPE_HALVES && mine) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (e0 + e < a.dim)
-                            px[e] = load_elem(x, row + (e0 + e >= half ? e0 + e - half : e0 + e + half), a.dtype);
-                }
-                load_angles<ROPE>(a, r, e0, mine, cc, ss);
-                rotate8<ROPE>(y, px, cc, ss, e0, half, a.dtype);
-            }
-            const u32x2 w = finish(s, y);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)  // (selects: the slot is not a constant here)
-                if (i == s) cw[i] = w;
-        }
-    }
-    if (kind != 1 || !mine) return;
-
-    // values: the 8 elements' codes of all 8 tokens are 64 (32) contiguous bytes of the tile; slots this
-    // call does not write keep their codes
-    if constexpr (kB8) {
+// Values: the 8 elements' codes of all 8 tokens are 64 (32) contiguous bytes of the tile; slots this call
+// does not write keep their codes.
+template <int FMT, int D>
+__device__ inline void store_values(uint8_t *codes, int in_page, int c, uint32_t live, u32x2 (&cw)[8]) {
+    if constexpr (FMT != CQKV_FMT_MXFP4) {
         uint8_t *dst = codes + (int64_t)in_page * 8 * D + 64 * c;
         transpose8x8(cw);
         if (live == 0xffu) {
@@ -464,16 +373,264 @@ __device__ inline void rows_unit(const PagedRowsArgs &a, const TileAt &t, int un
     }
 }
 
-// 4 wavefronts, one unit each; units of a tile are neighbours, so the wavefronts in flight together
-// read whole token rows.
-template <int FMT, int D, int ROPE, bool VEC>
-__global__ __launch_bounds__(256) void paged_append_kernel(PagedRowsArgs a) {
+// One head group of a tile.
+struct RowsUnit {
+    int kind, h;  // keys, values or queries; the lane's head
+    bool mine;
+    const void *x;
+    int64_t st, sh;
+};
+template <int D>
+__device__ inline RowsUnit rows_unit(const PagedRowsArgs &a, bool values, int u, int lane) {
+    constexpr int LPR = D / 8, RPW = 64 / LPR;
+    RowsUnit r;
+    r.kind = values ? 1 : u < a.k_units ? 0 : 2;
+    r.h = (r.kind == 2 ? u - a.k_units : u) * RPW + lane / LPR;
+    r.mine = r.h < (r.kind == 2 ? a.q_heads : a.kv_heads);
+    r.x = r.kind == 0 ? a.kx : r.kind == 1 ? a.vx : a.q;
+    r.st = r.kind == 0 ? a.k_st : r.kind == 1 ? a.v_st : a.q_st;
+    r.sh = r.kind == 0 ? a.k_sh : r.kind == 1 ? a.v_sh : a.q_sh;
+    return r;
+}
+
+// Slots that a wavefront takes: values all 8 of a tile; with angles 4, whose registers leave room for 4
+// wavefronts on a SIMD while the angles stay in them.
+template <int ROPE, bool VALUES>
+constexpr int rows_slots() { return ROPE != 0 && !VALUES ? 4 : 8; }
+
+// Slots sb .. sb + SL - 1 of a tile, for head groups [u0, u1): those of k (first) and q, or one of v.
+template <int FMT, int D, int ROPE, int VEC, bool VALUES>
+__device__ inline void rows_run(const PagedRowsArgs &a, const TileAt &t, int sb, int u0, int u1, int lane) {
+    constexpr int LPR = D / 8, SL = rows_slots<ROPE, VALUES>();
+    constexpr bool kRope = ROPE != 0 && !VALUES;
+    constexpr bool kB8 = FMT != CQKV_FMT_MXFP4;
+    const int c = lane % LPR, e0 = 8 * c, half = a.dim / 2;
+    const int s_lo = max(t.pos - 8 * t.tile - sb, 0), s_hi = min(t.pos + t.len - 8 * t.tile - sb, SL);
+    const int64_t row0 = t.first + (int64_t)8 * t.tile + sb - t.pos;  // packed row of slot sb
+
+    // the rows are requested before what has to be looked up for them (angles, the page)
+    u32x4 ca[SL], sa[SL], raw[SL], next[SL];
+    const auto load = [&](u32x4 (&w)[SL], const RowsUnit &r) {
+        const uint16_t *base = (const uint16_t *)r.x + r.h * r.sh + e0;
+#pragma unroll
+        for (int s = 0; s < SL; ++s) {
+            w[s] = u32x4{0u, 0u, 0u, 0u};
+            if (r.mine && e0 < a.dim && s >= s_lo && s < s_hi) w[s] = *(const u32x4 *)(base + (row0 + s) * r.st);
+        }
+    };
+    RowsUnit r = rows_unit<D>(a, VALUES, u0, lane);
+    if constexpr (VEC) {
+        load(raw, r);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    int page = 0;
+    const bool hole = (VALUES || u0 < a.k_units) && !page_of(a.pt, t.b, t.tile, page);
+    // the slots written: those of the call's rows, without the ones whose angles lie outside the tables
+    uint32_t live = 0;
+    int rows[SL][4];
+#pragma unroll
+    for (int s = 0; s < SL; ++s) {
+        if (s < s_lo || s >= s_hi) continue;
+        if (ROPE != 0 && !angle_rows(a, row0 + s, rows[s])) continue;
+        live |= 1u << s;
+    }
+    if (!live) return;
+    const int in_page = t.tile & ((1 << (a.pt.shift - 3)) - 1);  // the tile's place in its page
+    if (hole && (VALUES || u1 <= a.k_units)) return;  // (only queries are left)
+    const int64_t plane0 = (int64_t)(hole ? 0 : page) * a.kv_heads;
+
+    if constexpr (VEC) {
+        if constexpr (kRope) {
+#pragma unroll
+            for (int s = 0; s < SL; ++s) {
+                ca[s] = sa[s] = u32x4{0u, 0u, 0u, 0u};
+                if (!a.mixed && e0 < a.dim && ((live >> s) & 1)) load_angles<ROPE, false>(a, rows[s], e0, ca[s], sa[s]);
+            }
+            if (a.mixed) {  // element by element
+#pragma unroll 1
+                for (int s = 0; s < SL; ++s) {
+                    if (!((live >> s) & 1)) continue;
+                    int at[4];
+                    u32x4 cm = {0u, 0u, 0u, 0u}, sm = cm;
+                    angle_rows(a, row0 + s, at);
+                    if (e0 < a.dim) load_angles<ROPE, true>(a, at, e0, cm, sm);
+#pragma unroll
+                    for (int i = 0; i < SL; ++i)  // (selects: the slot is not a constant here)
+                        if (i == s) {
+                            ca[i] = cm;
+                            sa[i] = sm;
+                        }
+                }
+            }
+        }
+    }
+#pragma unroll 1
+    for (int u = u0; u < u1; ++u) {
+        RowsUnit rn = r;
+        if (kRope && u + 1 < u1) {
+            rn = rows_unit<D>(a, VALUES, u + 1, lane);
+            if constexpr (VEC) load(next, rn);
+        }
+        const int kind = r.kind, h = r.h;
+        const bool mine = r.mine && !(hole && kind != 2);
+        const PoolSide &side = VALUES ? a.v : a.k;
+        const int64_t plane = plane0 + (mine && kind != 2 ? h : 0);
+        uint8_t *codes = side.codes + plane * side.codes_plane, *scales = side.scales + plane * side.scales_plane;
+
+        // slot s's elements: the queries go out, keys and values are encoded
+        const auto finish = [&](int s, const float (&y)[8], auto any, bool &plain) {
+            u32x2 w = {0u, 0u};
+            if (!VALUES && kind == 2) {
+                if (!mine) return w;
+                const int64_t o = (row0 + s) * a.o_st + h * a.o_sh + e0;
+                if (VEC && e0 < a.dim) {
+                    u32x4 ow;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        ow[i] = VEC == 1 ? pack_bf16x2(y[2 * i], y[2 * i + 1]) : pack_f16x2(y[2 * i], y[2 * i + 1]);
+                    *(u32x4 *)((uint16_t *)a.q_out + o) = ow;
+                } else if (!VEC) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e0 + e < a.dim) store_elem(a.q_out, o + e, a.dtype, y[e]);
+                }
+                return w;
+            }
+            float tok = 0.0f;
+            uint32_t blk = 0;
+            plain = encode8<FMT, LPR, any.value>(y, w, tok, blk);
+            if (!mine) return w;
+            const int row = 8 * in_page + sb + s;
+            if constexpr (FMT == CQKV_FMT_FP8) {
+                if (c == 0) ((float *)scales)[row] = tok;
+            } else if ((c & 3) == 0) {
+                scales[row * (D / 32) + c / 4] = (uint8_t)blk;
+            }
+            if (!VALUES) {
+                if constexpr (kB8) *(u32x2 *)(codes + (int64_t)row * D + e0) = w;
+                else *(uint32_t *)(codes + (int64_t)row * (D / 2) + 4 * c) = w.x;
+            }
+            return w;
+        };
+
+        u32x2 cw[SL];
+        bool plain = true;
+        if constexpr (VEC) {
+            const auto row = [&](u32x4 w, u32x4 &cv, u32x4 &sv, float (&y)[8]) {
+                constexpr bool bf = VEC == 1;
+                raw_to_f32x8(w, bf, y);
+                if constexpr (kRope) {
+                    float px[8], cc[8], ss[8];
+                    // (converted here for every head group: as f32 across the loop they would take twice the registers)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(cv[i]), "+v"(sv[i]));
+                    if constexpr (ROPE == CQKV_ROPE_HALVES) {
+                        raw_to_f32x8(partner8<LPR>(w, a, e0, lane), bf, px);
+                        raw_to_f32x8(cv, bf, cc);
+                        raw_to_f32x8(sv, bf, ss);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) {
+                            const uint32_t cb = (cv[e / 4] >> (8 * (e & 2))) & 0xffffu, sb = (sv[e / 4] >> (8 * (e & 2))) & 0xffffu;
+                            cc[e] = bf ? bf16_bits_to_f32(cb) : f16_bits_to_f32(cb);
+                            ss[e] = bf ? bf16_bits_to_f32(sb) : f16_bits_to_f32(sb);
+                        }
+                    }
+                    rotate8<ROPE>(y, px, cc, ss, e0, half, bf ? CQKV_BF16 : CQKV_F16);
+                }
+            };
+            uint32_t again = 0;  // slots with a lane that needs the software encoders
+#pragma unroll
+            for (int s = 0; s < SL; ++s) {
+                cw[s] = u32x2{0u, 0u};
+                if (!((live >> s) & 1)) continue;
+                float y[8];
+                row(raw[s], ca[s], sa[s], y);
+                cw[s] = finish(s, y, std::false_type{}, plain);
+                if (__any(!plain)) again |= 1u << s;
+            }
+            if (__builtin_expect(again != 0, 0)) {
+                // (one copy of the encoders, which are long, for all slots: skipping a copy per slot costs an
+                // instruction fetch each, 4 us of a single token's 9)
+#pragma unroll 1
+                for (int s = 0; s < SL; ++s) {
+                    if (!((again >> s) & 1)) continue;
+                    u32x4 w = raw[0], cv = ca[0], sv = sa[0];
+#pragma unroll
+                    for (int i = 1; i < SL; ++i)
+                        if (i == s) {
+                            w = raw[i];
+                            cv = ca[i];
+                            sv = sa[i];
+                        }
+                    float y[8];
+                    row(w, cv, sv, y);
+                    const u32x2 r2 = finish(s, y, std::true_type{}, plain);
+#pragma unroll
+                    for (int i = 0; i < SL; ++i)
+                        if (i == s) cw[i] = r2;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < SL; ++s) cw[s] = u32x2{0u, 0u};
+#pragma unroll 1
+            for (int s = 0; s < SL; ++s) {
+                if (!((live >> s) & 1)) continue;
+                const int64_t row = (row0 + s) * r.st + h * r.sh;
+                float y[8];
+                load_any8(r.x, row, e0, mine ? a.dim : 0, a.dtype, y);
+                if constexpr (kRope) {
+                    int at[4];
+                    float px[8] = {}, cc[8], ss[8];
+                    angle_rows(a, row0 + s, at);
+                    if (ROPE == CQKV_ROPE_HALVES && mine) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            if (e0 + e < a.dim)
+                                px[e] = load_elem(r.x, row + (e0 + e >= half ? e0 + e - half : e0 + e + half), a.dtype);
+                    }
+                    load_angles_any<ROPE>(a, at, e0, mine, cc, ss);
+                    rotate8<ROPE>(y, px, cc, ss, e0, half, a.dtype);
+                }
+                const u32x2 w = finish(s, y, std::true_type{}, plain);
+#pragma unroll
+                for (int i = 0; i < SL; ++i)  // (selects: the slot is not a constant here)
+                    if (i == s) cw[i] = w;
+            }
+        }
+        if constexpr (VALUES) {
+            if (mine) store_values<FMT, D>(codes, in_page, c, live, cw);
+        }
+        if constexpr (!kRope) return;
+        r = rn;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int s = 0; s < SL; ++s) raw[s] = next[s];
+        }
+    }
+}
+
+// 4 wavefronts, one run of head groups each; runs of a tile are neighbours, so the wavefronts in flight
+// together read whole token rows.
+// VEC: rows of whole 16-byte pieces of bf16 (1) or f16 (2); 0: any dtype and strides.
+template <int FMT, int D, int ROPE, int VEC>
+__global__ __launch_bounds__(256, (VEC ? 4 : 1)) void paged_append_kernel(PagedRowsArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int at = (int)blockIdx.x * 4 + wave;
     const int idx = at / a.units;
     TileAt t;
     if (idx >= a.tiles || !find_tile(a.pt, a.positions, idx, lane, t)) return;
-    rows_unit<FMT, D, ROPE, VEC>(a, t, at - idx * a.units, lane);
+    // runs: of k and q for each part of the tile's slots, then of v
+    constexpr int SL = rows_slots<ROPE, false>(), PARTS = 8 / SL;
+    const int kq = a.k_units + a.q_units, kq_runs = (kq + a.per - 1) / a.per, run = at - idx * a.units;
+    if (run >= PARTS * kq_runs) {
+        const int u = run - PARTS * kq_runs;
+        rows_run<FMT, D, ROPE, VEC, true>(a, t, 0, u, u + 1, lane);
+    } else {
+        const int part = run / kq_runs, u0 = (run - part * kq_runs) * a.per;
+        rows_run<FMT, D, ROPE, VEC, false>(a, t, SL * part, u0, min(u0 + a.per, kq), lane);
+    }
 }
 
 // Read-back of one side: y = scale * value(code) in f32, rounded to the output dtype; rows of holes
@@ -498,23 +655,19 @@ __global__ __launch_bounds__(256) void paged_dequant_kernel(PagedRowsArgs a) {
     const uint8_t *codes = a.k.codes + plane * a.k.codes_plane;
     const uint8_t *scales = a.k.scales + plane * a.k.scales_plane;
     u32x2 cw[8];
-    float sc[8];
+    uint32_t sw[8];  // the rows' scales as they are in the pool (a conversion here would wait for each load)
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
         cw[s] = u32x2{0u, 0u};
-        sc[s] = 0.0f;
+        sw[s] = 0u;
     }
     if (!hole) {
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
             if (s < s_lo || s >= s_hi) continue;
             const int row = 8 * in_page + s;
-            if constexpr (FMT == CQKV_FMT_FP8) {
-                sc[s] = ((const float *)scales)[row];
-            } else {
-                const uint32_t b = scales[(int64_t)row * (D / 32) + c / 4];
-                sc[s] = b == 0 ? 0.0f : __uint_as_float(b << 23);
-            }
+            if constexpr (FMT == CQKV_FMT_FP8) sw[s] = ((const uint32_t *)scales)[row];
+            else sw[s] = scales[(int64_t)row * (D / 32) + c / 4];
             if (!a.side_is_value) {
                 if constexpr (kB8) cw[s] = *(const u32x2 *)(codes + (int64_t)row * D + e0);
                 else cw[s].x = *(const uint32_t *)(codes + (int64_t)row * (D / 2) + 4 * c);
@@ -543,16 +696,17 @@ __global__ __launch_bounds__(256) void paged_dequant_kernel(PagedRowsArgs a) {
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
         if (s < s_lo || s >= s_hi) continue;
+        const float sc = FMT == CQKV_FMT_FP8 ? __uint_as_float(sw[s]) : sw[s] == 0 ? 0.0f : __uint_as_float(sw[s] << 23);
         float y[8];
         if constexpr (kB8) {
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
                 const f32x2 p0 = __builtin_amdgcn_cvt_pk_f32_fp8(cw[s][w], false);
                 const f32x2 p1 = __builtin_amdgcn_cvt_pk_f32_fp8(cw[s][w], true);
-                y[4 * w] = p0.x * sc[s];
-                y[4 * w + 1] = p0.y * sc[s];
-                y[4 * w + 2] = p1.x * sc[s];
-                y[4 * w + 3] = p1.y * sc[s];
+                y[4 * w] = p0.x * sc;
+                y[4 * w + 1] = p0.y * sc;
+                y[4 * w + 2] = p1.x * sc;
+                y[4 * w + 3] = p1.y * sc;
             }
         } else {
             const uint32_t w = cw[s].x;
@@ -560,8 +714,8 @@ __global__ __launch_bounds__(256) void paged_dequant_kernel(PagedRowsArgs a) {
             const f32x2 p1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 1);
             const f32x2 p2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 2);
             const f32x2 p3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, 3);
-            y[0] = p0.x * sc[s]; y[1] = p0.y * sc[s]; y[2] = p1.x * sc[s]; y[3] = p1.y * sc[s];
-            y[4] = p2.x * sc[s]; y[5] = p2.y * sc[s]; y[6] = p3.x * sc[s]; y[7] = p3.y * sc[s];
+            y[0] = p0.x * sc; y[1] = p0.y * sc; y[2] = p1.x * sc; y[3] = p1.y * sc;
+            y[4] = p2.x * sc; y[5] = p2.y * sc; y[6] = p3.x * sc; y[7] = p3.y * sc;
         }
         const int64_t o = (row0 + s) * a.out_st + h * a.out_sh + e0;
         if (a.out_vec && a.out_dtype == CQKV_F32) {
@@ -583,8 +737,9 @@ __global__ __launch_bounds__(256) void paged_dequant_kernel(PagedRowsArgs a) {
 
 template <int FMT, int D, int ROPE>
 inline void launch_append(dim3 grid, hipStream_t st, const PagedRowsArgs &a) {
-    if (a.vec) hipLaunchKernelGGL((paged_append_kernel<FMT, D, ROPE, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((paged_append_kernel<FMT, D, ROPE, false>), grid, dim3(256), 0, st, a);
+    if (!a.vec) hipLaunchKernelGGL((paged_append_kernel<FMT, D, ROPE, 0>), grid, dim3(256), 0, st, a);
+    else if (a.dtype == CQKV_BF16) hipLaunchKernelGGL((paged_append_kernel<FMT, D, ROPE, 1>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_append_kernel<FMT, D, ROPE, 2>), grid, dim3(256), 0, st, a);
 }
 template <int FMT, int D>
 inline void launch_append_rope(int rope, dim3 grid, hipStream_t st, const PagedRowsArgs &a) {
