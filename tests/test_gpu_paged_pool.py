@@ -263,6 +263,78 @@ def test_rope_one_axis_is_the_dense_rope_append(cq, dev, kind):
         assert torch.equal(got, pack(cq.dequantize(dense, t, position=3)))
 
 
+@pytest.mark.parametrize("fmt", [FP8, MXFP8, MXFP4])
+@pytest.mark.parametrize("kind", [1, 2])
+def test_rope_special_values(cq, dev, fmt, kind):
+    """Infinities, zeros, subnormals and the largest values through the rotation: the codes are those of
+    the rotated rows."""
+    hq, hkv, d, page, n = 1, 2, 128, 32, 45
+    k, v = empty_pool(cq, dev, fmt, 2, hkv, d, page)
+    k2, v2 = copy_side(cq, k), copy_side(cq, v)
+    x = torch.randn(n, hq + 2 * hkv, d, generator=torch.Generator().manual_seed(1))
+    x[1, :, 70] = float("inf")
+    x[2, :, 5] = -float("inf")
+    x[3] = -0.0
+    x[4] = 1e-39
+    x[5] *= 1e-36
+    x[6, :, 9] = 3e38
+    x[13, 2, 3] = float("inf")
+    x[20] = 0.0
+    x = x.to(torch.bfloat16)
+    cos, sin = R.angle_tables(60, d, torch.bfloat16)
+    rp = torch.randint(1, 60, (2, n), generator=torch.Generator().manual_seed(2), dtype=torch.int32)
+    axes = cq.rope_sections((24, 40))
+    table, cu = R.make_table([n + 3], page, 2, dev, 1), R.prefix([n], dev)
+    xd = x.to(dev)
+    got = cq.paged_rope_append(k, v, xd[:, :hq], xd[:, hq:hq + hkv], xd[:, hq + hkv:], cos.to(dev),
+                               sin.to(dev), rp.to(dev), axes, table, cu, R.ints([3], dev), kind=kind)
+    assert torch.equal(got.cpu(), R.rope32(x[:, :hq], cos, sin, rp, axes, kind))
+    rot = R.rope32(x[:, hq:hq + hkv], cos, sin, rp, axes, kind)
+    assert not bool(rot.isnan().any())
+    dense_append(cq, k2, rot.to(dev), table, cu, [3])
+    dense_append(cq, v2, xd[:, hq + hkv:], table, cu, [3])
+    assert_same_pool(k, k2, hkv, d)
+    assert_same_pool(v, v2, hkv, d)
+
+
+@pytest.mark.parametrize("fmt,d,hq,hkv,dtype", [(FP8, 256, 14, 2, "bf16"), (MXFP4, 128, 17, 3, "f16"), (MXFP8, 64, 33, 9, "bf16")])
+def test_rope_long_call(cq, dev, fmt, d, hq, hkv, dtype):
+    """Calls so long that a wavefront takes two head groups (of k, of q, of both): holes keep their
+    queries, rows with an angle outside the tables are left out, an infinity in a key."""
+    page, lens, starts = 64, [5000, 1, 2000], [3, 900, 0]
+    kv = [s + n for s, n in zip(starts, lens)]
+    pages = sum(-(-n // page) for n in kv)
+    k, v = empty_pool(cq, dev, fmt, pages, hkv, d, page)
+    k2, v2 = copy_side(cq, k), copy_side(cq, v)
+    table, cu = R.make_table(kv, page, pages, dev, 4), R.prefix(lens, dev)
+    table[0, 7] = -1
+    total, dt = sum(lens), DTYPES[dtype]
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(total, hq + 2 * hkv, d, generator=g).to(dt)
+    x[77, hq, 3] = float("inf")
+    cos, sin = R.angle_tables(50, d, dt)
+    rp = torch.randint(1, 50, (2, total), generator=g, dtype=torch.int32)
+    axes = cq.rope_sections((16, d // 2 - 16))
+    rp[1, 1234] = 50
+    xd = x.to(dev)
+    out = torch.full((total, hq, d), 5.0, dtype=dt, device=dev)
+    cq.paged_rope_append(k, v, xd[:, :hq], xd[:, hq:hq + hkv], xd[:, hq + hkv:], cos.to(dev), sin.to(dev),
+                         rp.to(dev), axes, table, cu, R.ints(starts, dev), q_out=out)
+    rp[1, 1234] = 49
+    want = R.rope32(x[:, :hq], cos, sin, rp, axes, 1)
+    want[1234] = 5.0
+    assert torch.equal(out.cpu(), want)
+    rot = R.rope32(x[:, hq:hq + hkv], cos, sin, rp, axes, 1).to(dev)
+    # (the dense appends of the packed rows in front of and behind the one left out)
+    for a, b, first in ((0, 1234, 3), (1235, 5000, 3 + 1235)):
+        dense_append(cq, k2, rot[a:b], table, R.prefix([b - a], dev), [first])
+        dense_append(cq, v2, xd[a:b, hq + hkv:], table, R.prefix([b - a], dev), [first])
+    dense_append(cq, k2, rot[5000:], table[1:], R.prefix(lens[1:], dev), starts[1:])
+    dense_append(cq, v2, xd[5000:, hq + hkv:], table[1:], R.prefix(lens[1:], dev), starts[1:])
+    assert_same_pool(k, k2, hkv, d)
+    assert_same_pool(v, v2, hkv, d)
+
+
 def test_rope_positions_outside_the_tables(cq, dev):
     """A row with one angle outside the tables: q_out, k and v left as they were."""
     hq, hkv, d, page, n = 2, 1, 64, 32, 20
@@ -436,6 +508,32 @@ def test_attention_rows_outside_sequences(cq, dev):
 def test_attention_long_split(cq, dev):
     """Keys of one sequence split over the chip, next to short sequences in one split."""
     run_attention(cq, dev, FP8, 128, 4, 1, 64, "bf16", [1, 1, 2, 20], [5000, 3, 2500, 4000])
+
+
+PIECES = [
+    # fmt, d, hq, hkv, page, dtype, new, kv: planes that are cut into pieces, few and many of them, in calls of
+    # more than 64 sequences, with empty ones, of 1 to 4 column blocks, next to chunks
+    (FP8, 64, 4, 2, 32, "bf16", [1] * 70, [3000] + [1, 33, 64] * 22 + [0, 2000, 1100]),
+    (MXFP4, 64, 2, 2, 32, "f16", [1] * 60 + [0] * 10 + [2] * 75, [40] * 69 + [1500, 1100, 7000] + [3] * 73),
+    (MXFP8, 128, 4, 1, 64, "bf16", [9, 1, 16, 5], [5000, 1025, 1500, 5]),
+    (FP8, 128, 7, 1, 64, "f16", [9, 7, 1], [4000, 1300, 2100]),
+    (MXFP4, 128, 64, 8, 128, "bf16", [1, 1], [9000, 2000]),
+    (FP8, 256, 4, 2, 64, "bf16", [20, 1, 32], [3000, 1500, 1100]),
+    (MXFP8, 256, 2, 1, 32, "f16", [3, 0], [2500, 100]),
+    (FP8, 128, 8, 2, 64, "bf16", [100, 1, 9, 0, 40], [3000, 5000, 2500, 7, 1200]),
+    (FP8, 96, 3, 1, 64, "f16", [1, 6], [2500, 3300]),
+]
+
+
+@pytest.mark.parametrize("fmt,d,hq,hkv,page,dtype,new,kv", PIECES)
+def test_attention_pieces(cq, dev, fmt, d, hq, hkv, page, dtype, new, kv):
+    run_attention(cq, dev, fmt, d, hq, hkv, page, dtype, new, kv)
+
+
+@pytest.mark.parametrize("kw", [dict(window_left=1500), dict(causal=False, window_left=1300, window_right=40),
+                                dict(softcap=2.0)])
+def test_attention_pieces_masks(cq, dev, kw):
+    run_attention(cq, dev, MXFP8, 128, 8, 2, 64, "bf16", [1, 9, 1], [4000, 2500, 30], **kw)
 
 
 def test_attention_shared_pages(cq, dev):
@@ -645,3 +743,68 @@ def test_captured_step(cq, dev):
         lens += 1
         pos += 1
         table.copy_(table.roll(1, 0) if i == 1 else table)
+
+
+def test_captured_steps_share_a_workspace(cq, dev):
+    """Two graphs of one workspace (a decode step of cut planes and a chunk with single tokens beside it),
+    replayed in turn while lengths grow and shrink past every cut, with eager calls in between."""
+    hq, hkv, d, page, pages, b, top = 8, 2, 128, 64, 140, 3, 3000
+    k, v = R.make_pool(cq, dev, MXFP8, pages, hkv, d, page, 1)
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(1)).to(torch.int32)
+    table = torch.cat([table, table[:1]]).view(b, 47).to(dev)
+    lens = R.ints([1, 1, 1], dev)
+    x = torch.randn(202, hq, d, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(dev)
+    cus = [R.prefix([1] * b, dev), R.prefix([1, 200, 1], dev)]
+    most = [1, 200]
+    need = [cq.paged_attention_workspace_bytes(k, b, t, hq, m, top) for t, m in ((b, 1), (202, 200))]
+    assert min(need) > 0
+    ws = torch.full((max(need),), 0xff, dtype=torch.uint8, device=dev)
+    outs = [torch.zeros(t, hq, d, dtype=torch.bfloat16, device=dev) for t in (b, 202)]
+
+    def step(i, out, ws):
+        return cq.paged_attention(x[:out.shape[0]], k, v, table, cus[i], lens, most[i], top, 0.1, True, out=out,
+                                  workspace=ws)
+
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        for i in range(2):
+            step(i, outs[i], ws)
+    torch.cuda.current_stream().wait_stream(st)
+    graphs = []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            step(i, outs[i], ws)
+    for n in ([2900, 1500, 3], [1, 0, 2], [3000, 2999, 2998], [70, 205, 1100], [40, 3000, 1]):
+        lens.copy_(R.ints(n, dev))
+        for i in (0, 1, 0):
+            outs[i].fill_(7.0)
+            graphs[i].replay()
+            eager = step(i, torch.full_like(outs[i], 7.0), None)
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], eager)
+            assert bool(eager.isfinite().all())
+
+
+def test_two_calls_at_once(cq, dev):
+    """Calls on two streams over one pool, each with the library's own workspace."""
+    sides = R.make_pool(cq, dev, FP8, 160, 2, 128, 32, 1)
+    g = torch.Generator().manual_seed(1)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    args, wants = [], []
+    for i, n in enumerate((5000, 3100)):
+        table, cu = R.make_table([n], 32, 160, dev, i), R.prefix([1], dev)
+        q = torch.randn(1, 8, 128, generator=g).to(torch.bfloat16).to(dev)
+        args.append((q, *sides, table, cu, R.ints([n], dev), 1, 5000, 0.1, True))
+        wants.append(cq.paged_attention(*args[i]))
+    torch.cuda.synchronize()
+    gots = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                gots[i].append(cq.paged_attention(*args[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for got in gots[i]:
+            assert torch.equal(got, wants[i])
