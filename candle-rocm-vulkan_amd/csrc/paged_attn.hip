@@ -171,7 +171,10 @@ static PagedPlan paged_plan(int32_t d, int32_t batch, int32_t total, int32_t q_h
     // keys that a sequence's queries may see: the window's and the chunk's
     int64_t keys = max_kv;
     if (wl >= 0) keys = std::min<int64_t>(keys, (int64_t)wl + max_q + std::max(wr, 0));
-    p.from = 64;
+    // three blocks of 16 columns (16 sequences, FP8, bf16: D = 128, 4K keys, 32 columns 62 us against the chunk
+    // kernel's 83, 48 columns 86 and 94, 64 columns 101 and 79; D = 256, mixed lengths, 32 columns 73 and 114, 64
+    // columns 118 and 107)
+    p.from = 48;
     const bool many = cols > p.from;
     if (many && batch == 1) p.from = 0;  // the one sequence: no launch for short ones
     const int64_t rows = (int64_t)total * q_heads;
@@ -183,11 +186,12 @@ static PagedPlan paged_plan(int32_t d, int32_t batch, int32_t total, int32_t q_h
     };
     p.slot_cols = (int)((std::min<int64_t>(cols, p.from) + 15) / 16 * 16);
     if (keys > 32 * kPieceTiles && p.from) {
-        // one round of the chip's workgroups where the planes leave half of them to cut with (4 sequences of
-        // up to 128K keys, MXFP4, 64 / 8 heads: 88 us; three rounds: 132), else three, so that the last one is
-        // short (64 sequences of up to 8K keys, FP8, 32 / 8 heads: 129 us; one round of a plane each: 155)
+        // One round of the chip's workgroups where the planes leave most of them to cut with (4 sequences of up to
+        // 128K keys, MXFP4, 64 / 8 heads, 32 planes of 512 workgroups: 104 us; two rounds 115), else three, whose
+        // last is short (64 sequences of up to 8K keys, FP8, 32 / 8 heads, 512 planes: 136 us; a workgroup per
+        // plane 163). Half long and half short sequences: 192 planes 55 and 59 us, 256 planes 87 and 72.
         const int64_t slots = cus * (dk < 256 ? 2 : 1), planes = (int64_t)batch * kv_heads;
-        p.parts = (int)(2 * planes <= slots ? slots - planes : 3 * slots);
+        p.parts = (int)(8 * planes <= 3 * slots ? slots - planes : 3 * slots);
         // slots: at most 2 parts, and one more than the parts for every plane
         const int64_t cut = std::min<int64_t>(2 * p.parts, p.parts + planes);
         take(cut * p.slot_cols * dk);
