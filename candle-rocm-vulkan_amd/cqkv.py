@@ -945,7 +945,8 @@ def paged_attention(q: torch.Tensor, k_side: CacheSide, v_side: CacheSide, page_
     """Attention of packed queries (total, q_heads, D), bf16 or f16, over a page pool: sequence b's
     queries are the last of its first kv_lens[b] positions, whose keys are in the pool already.
     Single tokens, drafted tokens, chunks of prompts or a mixture. Masks, softcap and alibi_slopes as
-    flash_attn_varlen. Rows outside every sequence are not written."""
+    flash_attn_varlen. Rows outside every sequence are not written. A workspace (uint8) holds at least
+    paged_attention_workspace_bytes() bytes, whatever the lengths."""
     dev = _pool_device(k_side, v_side)
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
@@ -972,6 +973,8 @@ def paged_attention(q: torch.Tensor, k_side: CacheSide, v_side: CacheSide, page_
                                                    window_left, window_right)
         if n:
             workspace = _scratch(n, q.device)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise CqkvError(ERR_ARG, "workspace must be a contiguous tensor on the pool's device")
     ws, wsb = (None, 0) if workspace is None else (workspace.data_ptr(),
                                                    workspace.numel() * workspace.element_size())
     _check(L.cqkv_paged_attention(

@@ -206,12 +206,14 @@ static PagedPlan paged_plan(int32_t d, int32_t batch, int32_t total, int32_t q_h
         p.chunk_blocks = (int)std::min<int64_t>(all / nc + std::min<int64_t>(batch, all / (p.from + 1)), 1 << 24);
         const int64_t rest = std::max<int64_t>(all - cols, 0);
         const int64_t blocks = ((cols + nc - 1) / nc + (rest + nc - 1) / nc * (rest > (int64_t)p.from * (batch - 1))) * kv_heads;
-        // as many splits as end soonest: rounds of the chip over the length of a split
+        // as many splits as end soonest: rounds of the chip over the length of a split, and what its partials
+        // cost to write and merge, in tiles (64 keys of 256 columns take about 0.5 us, 4 MB at 8 TB/s)
         const int64_t ct = (keys + p.chunk_bk - 1) / p.chunk_bk + 1, slots = cus;
         int best = 1;
         double cost = 1e30;
         for (int cs = 1; cs <= 16 && (cs == 1 || ct / cs >= 8); ++cs) {
-            const double c = (double)((blocks * cs + slots - 1) / slots) * ((double)ct / cs + 4.0);
+            const double merge = cs > 1 ? (double)blocks * cs * nc * dk * 8 / 4e6 : 0.0;
+            const double c = (double)((blocks * cs + slots - 1) / slots) * ((double)ct / cs + 4.0) + merge;
             if (c < cost * 0.97) {
                 best = cs;
                 cost = c;
@@ -295,8 +297,9 @@ extern "C" int cqkv_paged_attention(const void *q, const int64_t q_strides[2], i
     a.dim = d;
     a.o_vec = d % 4 == 0 && (uintptr_t)out % 8 == 0 && a.o_st % 4 == 0 && a.o_sh % 4 == 0;
     a.q_vec = d % 8 == 0 && (uintptr_t)q % 16 == 0 && a.q_st % 8 == 0 && a.q_sh % 8 == 0;
-    a.wl = window_left;
-    a.wr = window_right;
+    // (windows past every position, so that sums with positions stay in 32 bits)
+    a.wl = std::min(window_left, 1 << 30);
+    a.wr = std::min(window_right, (1 << 30) - 1);
     a.scale_log2 = softmax_scale * kLog2e;
     a.cap2 = softcap * kLog2e;
     a.alibi = alibi_slopes;
@@ -325,6 +328,7 @@ extern "C" int cqkv_paged_attention(const void *q, const int64_t q_strides[2], i
     if (p.total) {
         if (ws && workspace_bytes < p.total)
             return fail(CQKV_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", who, workspace_bytes, p.total);
+        if ((uintptr_t)ws % 16) return fail(CQKV_ERR_ARG, "%s: workspace not 16-byte aligned", who);
         if (!ws) {
             CQKV_HIP_CHECK(hipMallocAsync(&ws, p.total, st));
             owned = true;

@@ -7,7 +7,7 @@
  * and returning CQKV_OK or a negative status; cqkv_last_error() gives the message of the last
  * failure of the calling thread. Device memory is allocated (stream-ordered, hipMallocAsync /
  * hipFreeAsync on the call's stream) only by: cqkv_decode_attention,
- * cqkv_decode_attention_paged, cqkv_flash_attn_ext, cqkv_flash_attn_blocks and
+ * cqkv_decode_attention_paged, cqkv_flash_attn_ext, cqkv_flash_attn_blocks, cqkv_paged_attention and
  * cqkv_dequantize_rows when they are given no workspace (each has a *_workspace_bytes query);
  * cqkv_flash_attn (its workspace); cqkv_flash_attn_fp8 given no workspace (the staged K / V and
  * the attention's workspace); cqkv_quant_append, cqkv_rope_quant_append and the cache append of
@@ -525,8 +525,9 @@ int cqkv_side_copy(const cqkv_side *dst, const cqkv_side *src, int32_t batch, in
  * into the `total` rows. Position p of sequence b lies in page table[b * table_stride + p / page size].
  * Page ids outside [0, n_pages), and positions past the table's max_pages pages, are holes: rows
  * appended there are dropped, they read back as zeros and their keys are masked. Sequences may share
- * pages that they only read (a common prefix, the same page twice); two rows of one call appended to
- * one position of one page, by two sequences that share it, leave a mixture of both.
+ * pages that they only read (a common prefix, the same page twice); where one call appends to the same
+ * 8-position tile of a page for two sequences, the codes left there are undefined (every address is in
+ * the pool all the same).
  * The arrays are read on the device, in stream order. The calls allocate nothing but the workspace
  * of cqkv_paged_attention when none is given. */
 typedef struct cqkv_pages {
@@ -580,7 +581,11 @@ int cqkv_paged_dequantize(const cqkv_side *side, const cqkv_pages *pages, const 
  * as cqkv_decode_attention (causal: window_right 0). max_q_len / max_kv_len: the longest sequences
  * (host), which size the launch; queries past max_q_len are not computed. Rows without a visible key
  * are zeros. Keys that a query does not see never reach its row, whatever their bytes.
- * workspace: at least cqkv_paged_attention_workspace_bytes() (0: none needed); NULL = allocated
+ * Up to 48 columns per kv head (queries times the heads of a group) K and V enter the products exactly;
+ * sequences of more take a dequantized value rounded to `dtype` (f16: infinite past 65504), as prefill
+ * over a read-back cache does.
+ * workspace: at least cqkv_paged_attention_workspace_bytes() (0: none needed), 16-byte aligned; it does
+ * not depend on the lengths, and calls in one stream may share it, captured ones too. NULL = allocated
  * (stream-ordered) and freed by the call. */
 size_t cqkv_paged_attention_workspace_bytes(const cqkv_side *k_side, int32_t batch, int32_t total,
                                             int32_t q_heads, int32_t max_q_len, int32_t max_kv_len,

@@ -536,6 +536,26 @@ def test_attention_pieces_masks(cq, dev, kw):
     run_attention(cq, dev, MXFP8, 128, 8, 2, 64, "bf16", [1, 9, 1], [4000, 2500, 30], **kw)
 
 
+@pytest.mark.parametrize("new,kv", [([1, 9, 30], [40, 2000, 20]), ([100, 30], [300, 20])])
+def test_attention_widest_windows(cq, dev, new, kv):
+    """Windows of the largest 32-bit values (also of queries in front of the first key) are no windows."""
+    most = 2 ** 31 - 1
+    run_attention(cq, dev, FP8, 64, 4, 2, 32, "bf16", new, kv, causal=False, window_left=most, window_right=most)
+    run_attention(cq, dev, FP8, 64, 4, 2, 32, "bf16", new, kv, window_left=most)
+
+
+def test_attention_workspace_of_another_device_or_alignment(cq, dev):
+    sides = R.make_pool(cq, dev, FP8, 80, 2, 128, 32, 1)
+    table, cu = R.make_table([2500], 32, 80, dev, 1), R.prefix([1], dev)
+    q = torch.zeros(1, 8, 128, dtype=torch.bfloat16, device=dev)
+    args = (q, *sides, table, cu, R.ints([2500], dev), 1, 2500, 0.1, True)
+    n = cq.paged_attention_workspace_bytes(sides[0], 1, 1, 8, 1, 2500)
+    for ws in (torch.zeros(n, dtype=torch.uint8), torch.zeros(n + 1, dtype=torch.uint8, device=dev)[1:],
+               torch.zeros(2 * n, dtype=torch.uint8, device=dev)[::2]):
+        with pytest.raises(cq.CqkvError):
+            cq.paged_attention(*args, workspace=ws)
+
+
 def test_attention_shared_pages(cq, dev):
     """Two sequences over the same pages, and one that holds a page twice."""
     sides = R.make_pool(cq, dev, FP8, 3, 2, 64, 32, 1)

@@ -118,6 +118,12 @@ def test_small_workspace_is_refused(cq):
     assert attend(cq, p=p, total=1, max_q=1, max_kv=4096, ws=BAD, ws_bytes=need - 1) == cq.ERR_WORKSPACE
 
 
+def test_misaligned_workspace_is_refused(cq):
+    need = cq.lib().cqkv_paged_attention_workspace_bytes(ctypes.byref(side(cq)), 1, 1, 4, 1, 4096, -1, 0)
+    p = pages(cq, batch=1, max_pages=64, stride=64)
+    assert attend(cq, p=p, total=1, max_q=1, max_kv=4096, ws=BAD + 8, ws_bytes=need + 8) == cq.ERR_ARG
+
+
 @pytest.mark.parametrize("call", [append, rope, read, attend])
 def test_nothing_to_do(cq, call):
     """No rows, or no sequences: the arguments are checked, nothing is launched."""
