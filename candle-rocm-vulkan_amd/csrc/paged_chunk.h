@@ -5,13 +5,16 @@
 // The pages' codes become MFMA operands of the queries' dtype once per workgroup: every thread loads 16
 // codes of K and 16 of V of a 64-key tile and writes them to LDS as operands: keys exactly (E4M3 codes as
 // they are, their f32 scale multiplies the scores; MX codes times their power of two), values times their
-// scales, rounded to the dtype as a dequantized cache holds them; K rows in the order that makes the S^T registers of a lane whole groups of 8 keys (key
-// bits 2 and 3 exchanged), V^T rows of 8-key chunks straight from the pool's 8-token tiles. From there it
+// scales, rounded to the dtype as a dequantized cache holds them; K rows in the order that
+// makes the S^T registers of a lane whole groups of 8 keys (key bits 2 and 3 exchanged), V^T rows of 8-key
+// chunks straight from the pool's 8-token tiles. From there it
 // is the dense prefill's core: S^T(t + 1) on the MFMA pipe while the VALU exponentiates S(t), then
 // O^T += V^T(t) P^T(t) while it sums P(t) and takes the maxima of S(t + 1). Two LDS stages each: step t
 // reads K(t + 1) and V(t) and writes K(t + 2) and V(t + 1), whose codes were requested a step before.
 // Bound by the MFMA and VALU work of the softmax; the conversion costs about 64 VALU instructions of a
 // wavefront per tile beside the softmax's 110 and 32 exponentials.
+// 512 tokens against 16K keys, FP8, 32 / 8 heads, D = 128: 157 us under the profiler, 0.86 PFLOP/s (151 us for a
+// call with its merge); 1023 tokens against 7K keys, MXFP8: 139 us.
 #pragma once
 
 #include "paged_attn.h"

