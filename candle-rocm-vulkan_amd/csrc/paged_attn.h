@@ -127,7 +127,7 @@ __device__ inline uint32_t piece_tiles(const PagedAttnArgs &a, int lane) {
         total += wave_sum_u32((uint32_t)max(seq_tiles(a, paged_seq_lane(a, i + lane)), 0));  // (each at most 2^25)
     }
     const uint64_t u = (total * (uint32_t)a.kv_heads + (uint32_t)a.parts - 1) / (uint32_t)a.parts;
-    return (uint32_t)min(max(u, (uint64_t)kPieceTiles), (uint64_t)0x40000000u);
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)min(max(u, (uint64_t)kPieceTiles), (uint64_t)0x40000000u));
 }
 __device__ inline SeqWork seq_work(const PagedAttnArgs &a, const PagedSeq &s, uint32_t u) {
     const int n = seq_tiles(a, s);
@@ -175,8 +175,8 @@ __device__ inline PageRsrc page_rsrc(const PagedAttnArgs &a, int page, int hk, b
 }
 
 // Code loads: read once per call (nontemporal), or by other wavefronts on the same tile too (ONCE false:
-// they then come from L2; nontemporal lines come from HBM again. 16 sequences of 5 drafted tokens, FP8: 55 us
-// against 61; single tokens, read once: 145 against 135).
+// they then come from L2; nontemporal lines come from HBM again). 16 sequences of 5 drafted tokens, FP8: 47 us,
+// 56 with ONCE; single tokens of 64 sequences: 128 with ONCE, 138 without or with a branch between the two.
 template <bool ONCE>
 __device__ inline u32x4 code128(rsrc_t r, uint32_t off) { return ONCE ? ld128_stream(r, off) : ld128(r, off); }
 template <bool ONCE>
@@ -532,10 +532,10 @@ __device__ inline u32x4 paged_q8(const uint16_t *row, int d0, int dim, bool vec)
 }
 
 // Tiles in flight per wavefront: as many as leave two wavefronts to a SIMD (MXFP4, D = 128, 4 sequences of up to
-// 128K keys: 107 us with two, 104 with three; one short sequence at D = 64: 11.8 with two, 10.9 with four).
+// 128K keys: 100 us with two, 88 with three; one short sequence at D = 64: 14 with two, 11.7 with four).
 constexpr int paged_sets(int fmt, int d) { return d == 64 ? 4 : d == 128 && fmt == CQKV_FMT_MXFP4 ? 3 : 2; }
 
-template <int FMT, int D, bool F16>
+template <int FMT, int D, bool F16, bool ONCE>
 __global__ __launch_bounds__(256, (D < 256 ? 2 : 1)) void paged_attn_kernel(PagedAttnArgs a) {
     constexpr int NCH = D / 32, WAVES = 4, NS = paged_sets(FMT, D);
     __shared__ __attribute__((aligned(16))) float sm_o[WAVES][16][D + 4];
@@ -569,6 +569,11 @@ __global__ __launch_bounds__(256, (D < 256 ? 2 : 1)) void paged_attn_kernel(Page
         }
         if (b < 0) return;
     }
+    // (uniform, which the compiler does not see through the sums over lanes: the pages' resources must be
+    // scalars, or every load becomes a loop over the lanes' values)
+    b = __builtin_amdgcn_readfirstlane(b);
+    rest = __builtin_amdgcn_readfirstlane(rest);
+    slot = __builtin_amdgcn_readfirstlane(slot);
     const PagedSeq sq = paged_seq(a, b);
     int hk = rest, tb = sq.t0, te = sq.t1;
     if (a.parts == 0) {
@@ -595,8 +600,7 @@ __global__ __launch_bounds__(256, (D < 256 ? 2 : 1)) void paged_attn_kernel(Page
     const auto page_id = [&](int i) { return i < te ? table[i >> tshift] : -1; };
     const auto load = [&](PagedTile<FMT, D> &r, int i, int id) {
         const PageRsrc p = page_rsrc(a, id, hk, (uint32_t)id < (uint32_t)a.pt.n_pages);
-        if (cshift == 0) paged_load<FMT, D, true>(r, p, 32u * (uint32_t)(i & tmask), lane);
-        else paged_load<FMT, D, false>(r, p, 32u * (uint32_t)(i & tmask), lane);
+        paged_load<FMT, D, ONCE>(r, p, 32u * (uint32_t)(i & tmask), lane);
     };
     int page[NS];
 #pragma unroll
@@ -710,23 +714,22 @@ __global__ __launch_bounds__(256, (D < 256 ? 2 : 1)) void paged_attn_kernel(Page
     }
 }
 
+template <int FMT, int D>
+inline void launch_paged_attn_d(bool f16, bool once, dim3 grid, hipStream_t st, const PagedAttnArgs &a) {
+    if (f16 && once) hipLaunchKernelGGL((paged_attn_kernel<FMT, D, true, true>), grid, dim3(256), 0, st, a);
+    else if (f16) hipLaunchKernelGGL((paged_attn_kernel<FMT, D, true, false>), grid, dim3(256), 0, st, a);
+    else if (once) hipLaunchKernelGGL((paged_attn_kernel<FMT, D, false, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_attn_kernel<FMT, D, false, false>), grid, dim3(256), 0, st, a);
+}
 template <int FMT>
-inline void launch_paged_attn(int dk, bool f16, dim3 grid, hipStream_t st, const PagedAttnArgs &a) {
-#define CQKV_LAUNCH(D)                                                                                        \
-    if (f16) hipLaunchKernelGGL((paged_attn_kernel<FMT, D, true>), grid, dim3(256), 0, st, a);                \
-    else hipLaunchKernelGGL((paged_attn_kernel<FMT, D, false>), grid, dim3(256), 0, st, a)
-    if (dk == 64) {
-        CQKV_LAUNCH(64);
-    } else if (dk == 128) {
-        CQKV_LAUNCH(128);
-    } else {
-        CQKV_LAUNCH(256);
-    }
-#undef CQKV_LAUNCH
+inline void launch_paged_attn(int dk, bool f16, bool once, dim3 grid, hipStream_t st, const PagedAttnArgs &a) {
+    if (dk == 64) launch_paged_attn_d<FMT, 64>(f16, once, grid, st, a);
+    else if (dk == 128) launch_paged_attn_d<FMT, 128>(f16, once, grid, st, a);
+    else launch_paged_attn_d<FMT, 256>(f16, once, grid, st, a);
 }
 
 #define CQKV_PAGED_ATTN_LAUNCHER(F) \
-    void paged_attn_launch_##F(int dk, bool f16, dim3 grid, hipStream_t st, const PagedAttnArgs &a);
+    void paged_attn_launch_##F(int dk, bool f16, bool once, dim3 grid, hipStream_t st, const PagedAttnArgs &a);
 CQKV_PAGED_ATTN_LAUNCHER(2)
 CQKV_PAGED_ATTN_LAUNCHER(4)
 CQKV_PAGED_ATTN_LAUNCHER(5)

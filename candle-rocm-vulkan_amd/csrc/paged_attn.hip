@@ -161,6 +161,7 @@ static int paged_cus() {
 // ones the chunk kernel.
 struct PagedPlan {
     int parts, slot_cols;
+    bool once;  // a tile is read by one wavefront in most sequences of the decode kernel
     int from, chunk_blocks, chunk_splits, chunk_tps, chunk_bk;
     size_t part_lse, chunk_o, chunk_lse, total;  // workspace offsets and size
 };
@@ -172,11 +173,14 @@ static PagedPlan paged_plan(int32_t d, int32_t batch, int32_t total, int32_t q_h
     // keys that a sequence's queries may see: the window's and the chunk's
     int64_t keys = max_kv;
     if (wl >= 0) keys = std::min<int64_t>(keys, (int64_t)wl + max_q + std::max(wr, 0));
-    // three blocks of 16 columns (16 sequences, FP8, bf16: D = 128, 4K keys, 32 columns 62 us against the chunk
-    // kernel's 83, 48 columns 86 and 94, 64 columns 101 and 79; D = 256, mixed lengths, 32 columns 73 and 114, 64
-    // columns 118 and 107)
-    p.from = 48;
+    // three blocks of 16 columns, four at D = 256 (16 sequences, FP8, bf16: D = 128, 4K keys, 32 columns 55 us
+    // against the chunk kernel's 78, 48 columns 81 and 82, 64 columns 88 and 72; D = 256, up to 8K keys, 64
+    // columns 99 and 107)
+    p.from = dk == 256 ? 64 : 48;
     const bool many = cols > p.from;
+    // (next to a long sequence: the tokens that the others have on average)
+    const int64_t others = batch > 1 ? (std::max(total - max_q, 1) + batch - 2) / (batch - 1) : 1;
+    p.once = (many ? others * group : cols) <= 16;
     if (many && batch == 1) p.from = 0;  // the one sequence: no launch for short ones
     const int64_t rows = (int64_t)total * q_heads;
     size_t at = 0;
@@ -188,9 +192,9 @@ static PagedPlan paged_plan(int32_t d, int32_t batch, int32_t total, int32_t q_h
     p.slot_cols = (int)((std::min<int64_t>(cols, p.from) + 15) / 16 * 16);
     if (keys > 32 * kPieceTiles && p.from) {
         // One round of the chip's workgroups where the planes leave most of them to cut with (4 sequences of up to
-        // 128K keys, MXFP4, 64 / 8 heads, 32 planes of 512 workgroups: 104 us; two rounds 115), else three, whose
-        // last is short (64 sequences of up to 8K keys, FP8, 32 / 8 heads, 512 planes: 136 us; a workgroup per
-        // plane 163). Half long and half short sequences: 192 planes 55 and 59 us, 256 planes 87 and 72.
+        // 128K keys, MXFP4, 64 / 8 heads, 32 planes of 512 workgroups: 87 us; two rounds 114), else three, whose
+        // last is short (64 sequences of up to 8K keys, FP8, 32 / 8 heads, 512 planes: 137 us; longer pieces 151).
+        // Half long and half short sequences: 192 planes 53 and 56 us, 256 planes 84 and 68.
         const int64_t slots = cus * (dk < 256 ? 2 : 1), planes = (int64_t)batch * kv_heads;
         p.parts = (int)(8 * planes <= 3 * slots ? slots - planes : 3 * slots);
         // slots: at most 2 parts, and one more than the parts for every plane
@@ -352,9 +356,9 @@ extern "C" int cqkv_paged_attention(const void *q, const int64_t q_strides[2], i
     }
     if (e == hipSuccess && wgs) {
         const dim3 grid((unsigned)wgs);
-        if (k_side->format == CQKV_FMT_FP8) paged_attn_launch_5(dk, f16, grid, st, a);
-        else if (k_side->format == CQKV_FMT_MXFP8) paged_attn_launch_4(dk, f16, grid, st, a);
-        else paged_attn_launch_2(dk, f16, grid, st, a);
+        if (k_side->format == CQKV_FMT_FP8) paged_attn_launch_5(dk, f16, p.once, grid, st, a);
+        else if (k_side->format == CQKV_FMT_MXFP8) paged_attn_launch_4(dk, f16, p.once, grid, st, a);
+        else paged_attn_launch_2(dk, f16, p.once, grid, st, a);
         e = hipGetLastError();
     }
     if (e == hipSuccess && p.total) {

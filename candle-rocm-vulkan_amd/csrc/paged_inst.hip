@@ -22,9 +22,9 @@ void CQKV_CAT(paged_dequant_launch_, CQKV_PAGED_FMT)(int dk, dim3 grid, hipStrea
     launch_dequant<CQKV_PAGED_FMT>(dk, grid, st, a);
 }
 
-void CQKV_CAT(paged_attn_launch_, CQKV_PAGED_FMT)(int dk, bool f16, dim3 grid, hipStream_t st,
+void CQKV_CAT(paged_attn_launch_, CQKV_PAGED_FMT)(int dk, bool f16, bool once, dim3 grid, hipStream_t st,
                                                  const PagedAttnArgs &a) {
-    launch_paged_attn<CQKV_PAGED_FMT>(dk, f16, grid, st, a);
+    launch_paged_attn<CQKV_PAGED_FMT>(dk, f16, once, grid, st, a);
 }
 
 void CQKV_CAT(paged_chunk_launch_, CQKV_PAGED_FMT)(int dk, bool f16, bool logit, dim3 grid,

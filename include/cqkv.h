@@ -581,7 +581,7 @@ int cqkv_paged_dequantize(const cqkv_side *side, const cqkv_pages *pages, const 
  * as cqkv_decode_attention (causal: window_right 0). max_q_len / max_kv_len: the longest sequences
  * (host), which size the launch; queries past max_q_len are not computed. Rows without a visible key
  * are zeros. Keys that a query does not see never reach its row, whatever their bytes.
- * Up to 48 columns per kv head (queries times the heads of a group) K and V enter the products exactly;
+ * Up to 48 columns per kv head (queries times the heads of a group; 64 above D = 128) K and V enter the products exactly;
  * sequences of more take a dequantized value rounded to `dtype` (f16: infinite past 65504), as prefill
  * over a read-back cache does.
  * workspace: at least cqkv_paged_attention_workspace_bytes() (0: none needed), 16-byte aligned; it does

@@ -126,7 +126,7 @@ def assert_call(out, q, kvals, vvals, table, cu, kv, scale, dtype, fmt4, **kw):
     group, d = q.shape[1] // kvals.shape[1], q.shape[2]
     many = torch.zeros_like(wrote)
     for a, b in zip(cu.tolist(), cu.tolist()[1:]):
-        many[a:b] = (b - a) * group > 48
+        many[a:b] = (b - a) * group > (64 if d > 128 else 48)
     for rows, chunk in ((wrote & ~many, False), (wrote & many, True)):
         if rows.any():
             used = [page_rows(kvals, table, b, n) for b, n in enumerate(kv) if n]
