@@ -17,9 +17,9 @@
 // registers of one block, and two fit a SIMD.
 //
 // Bound by HBM for single tokens over 8-bit codes (64 sequences of up to 8K keys, FP8, 32 / 8 heads, D = 128:
-// 131 us, 5.2 TB/s), by the decoding VALU work for MXFP4 (4 sequences of up to 128K keys, 64 / 8 heads: 98 us,
-// 4.7 TB/s), by the latency of a tile for drafted tokens (16 sequences of 5: 49 us, 2.6 TB/s), by the chain
-// length -> page -> tile -> merge for a short sequence (9.5 us at 500 keys, D = 64).
+// 119 us, 5.7 TB/s), by the decoding VALU work for MXFP4 (4 sequences of up to 128K keys, 64 / 8 heads: 85 us,
+// 5.4 TB/s), by the latency of a tile for drafted tokens (16 sequences of 5: 40 us, 3.1 TB/s), by the chain
+// length -> page -> tile -> merge for a short sequence (7.6 us at 500 keys, D = 64).
 #pragma once
 
 #include <type_traits>
