@@ -101,12 +101,7 @@ struct SeqWork {
 __device__ inline int seq_tiles(const PagedAttnArgs &a, const PagedSeq &s) {  // -1: not the decode kernel's
     return s.lq > 0 && !chunk_takes(a, s) ? max(s.t1 - s.t0, 0) : -1;
 }
-__device__ inline uint32_t wave_sum_u32(uint32_t v) {
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) v += (uint32_t)__shfl_xor((int)v, m);
-    return v;
-}
-// Inclusive sum over the lanes of two counts, in the halves of a word.
+// Inclusive sum over the lanes (of a count, or of two in the halves of a word).
 __device__ inline uint64_t wave_scan2(uint64_t v, int lane) {
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) {
@@ -121,11 +116,8 @@ __device__ inline uint64_t readlane64(uint64_t v, int l) {
 }
 // U: at least kPieceTiles tiles, so that a piece's start and merge (about 3 us) stay small beside it.
 constexpr int kPieceTiles = 32;
-__device__ inline uint32_t piece_tiles(const PagedAttnArgs &a, int lane) {
-    uint64_t total = 0;
-    for (int i = 0; i < a.pt.batch; i += 64) {
-        total += wave_sum_u32((uint32_t)max(seq_tiles(a, paged_seq_lane(a, i + lane)), 0));  // (each at most 2^25)
-    }
+__device__ inline uint32_t piece_tiles(const PagedAttnArgs &a, uint64_t lane_tiles, int lane) {
+    const uint64_t total = readlane64(wave_scan2(lane_tiles, lane), 63);
     const uint64_t u = (total * (uint32_t)a.kv_heads + (uint32_t)a.parts - 1) / (uint32_t)a.parts;
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)min(max(u, (uint64_t)kPieceTiles), (uint64_t)0x40000000u));
 }
@@ -137,6 +129,38 @@ __device__ inline SeqWork seq_work(const PagedAttnArgs &a, const PagedSeq &s, ui
 __device__ inline uint64_t seq_pieces(const PagedAttnArgs &a, const SeqWork &w) {
     const uint32_t p = (uint32_t)(w.pieces * a.kv_heads);
     return (uint64_t)(w.pieces > 1 ? p : 0u) << 32 | p;
+}
+
+// Sequence of piece `idx` of the call (-1: past the last) and the pieces in front of that sequence. A lane
+// sums a run of sequences, so the search costs two scans and a run's loads, which are independent, however
+// many sequences there are.
+__device__ inline int piece_sequence(const PagedAttnArgs &a, uint32_t idx, int lane, uint32_t &u, uint64_t &first) {
+    const int run = (a.pt.batch + 63) >> 6;
+    uint64_t mine = 0;
+#pragma unroll 4
+    for (int i = 0; i < run; ++i) mine += (uint32_t)max(seq_tiles(a, paged_seq_lane(a, lane * run + i)), 0);
+    u = piece_tiles(a, mine, lane);
+    mine = 0;
+#pragma unroll 4
+    for (int i = 0; i < run; ++i) mine += seq_pieces(a, seq_work(a, paged_seq_lane(a, lane * run + i), u));
+    uint64_t sum = wave_scan2(mine, lane), past = __ballot((uint32_t)sum > idx);
+    if (!past) return -1;
+    const int l = __builtin_ctzll(past);
+    first = readlane64(sum - mine, l);
+    if (run == 1) return l;
+    for (int base = l * run; base < (l + 1) * run; base += 64) {  // the lane's run, a sequence per lane
+        const int b = base + lane;
+        mine = b < (l + 1) * run ? seq_pieces(a, seq_work(a, paged_seq_lane(a, b), u)) : 0;
+        sum = first + wave_scan2(mine, lane);
+        past = __ballot((uint32_t)sum > idx);
+        if (past) {
+            const int k = __builtin_ctzll(past);
+            first = readlane64(sum - mine, k);
+            return base + k;
+        }
+        first = readlane64(sum, 63);
+    }
+    return -1;
 }
 
 // Head dim held in k-slot 0 of MFMA chunk j by lane group g (the same for K and Q operands).
@@ -551,21 +575,11 @@ __global__ __launch_bounds__(256, (D < 256 ? 2 : 1)) void paged_attn_kernel(Page
         b = (int)blockIdx.x / a.kv_heads;
         rest = (int)blockIdx.x % a.kv_heads;
     } else {
-        u = piece_tiles(a, lane);
-        uint64_t before = 0;
-        for (int base = 0; base < a.pt.batch; base += 64) {
-            const uint64_t mine = seq_pieces(a, seq_work(a, paged_seq_lane(a, base + lane), u));
-            const uint64_t sum = before + wave_scan2(mine, lane);
-            const uint64_t past = __ballot((uint32_t)sum > blockIdx.x);
-            if (past) {
-                const int l = __builtin_ctzll(past);
-                b = base + l;
-                const uint64_t first = readlane64(sum - mine, l);
-                rest = (int)(blockIdx.x - (uint32_t)first);
-                slot = (int)(first >> 32) + rest;
-                break;
-            }
-            before = readlane64(sum, 63);
+        uint64_t first = 0;
+        b = piece_sequence(a, blockIdx.x, lane, u, first);
+        if (b >= 0) {
+            rest = (int)(blockIdx.x - (uint32_t)first);
+            slot = (int)(first >> 32) + rest;
         }
         if (b < 0) return;
     }

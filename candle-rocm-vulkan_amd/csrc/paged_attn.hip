@@ -8,8 +8,7 @@ namespace cqkv {
 // Merge of the pieces: o = sum_s w_s o_s / sum_s w_s, w_s = 2^(lse_s - max lse). A row outside every
 // sequence, past max_q of its sequence, or written whole by its only workgroup is left alone.
 //
-// Bound by latency: the row's sequence has to be found (prefix sums, 64 sequences at a time), then its
-// pieces. D / 4 lanes take a row, so a wavefront has 256 / D heads of a token at once. Few rows (DEEP): a
+// Bound by latency: the row's sequence and its slots have to be found, then its pieces. D / 4 lanes take a row, so a wavefront has 256 / D heads of a token at once. Few rows (DEEP): a
 // workgroup for them, its 8 wavefronts taking the pieces 8 at a time. Many rows: a wavefront takes `per`
 // such groups of a token, so the sequence is found once for them, two in flight. 256 rows of up to 20 pieces:
 // 4.9 us (a wavefront per row 21); 33472 rows of 2: 13 us (33).
@@ -21,23 +20,27 @@ __global__ __launch_bounds__(DEEP ? 512 : 256) void paged_combine_kernel(PagedAt
     const int groups = (a.q_heads + RW - 1) / RW, runs = (groups + per - 1) / per;
     const int token = idx / runs, g0 = (idx - token * runs) * per, g1 = min(g0 + per, groups);
     if (token >= a.pt.total) return;
-    // the sequence, and the slots in front of its
-    const uint32_t u = a.parts ? piece_tiles(a, lane) : 0x40000000u;
+    // the sequence, and the slots in front of its; sequences in steps of 64, whose loads are independent
+    const int batch = a.pt.batch;
     int b = -1;
-    uint32_t slots = 0;
-    for (int base = 0; base < a.pt.batch; base += 64) {
-        const PagedSeq ls = paged_seq_lane(a, base + lane);
-        const uint64_t at = __ballot(token >= ls.first && token < ls.first + ls.lq);
-        const uint32_t mine = (uint32_t)(seq_pieces(a, seq_work(a, ls, u)) >> 32);
-        if (at) {
-            const int l = __builtin_ctzll(at);
-            b = base + l;
-            slots += wave_sum_u32(lane < l ? mine : 0u);
-            break;
-        }
-        slots += wave_sum_u32(mine);
+    uint64_t tiles = 0;
+#pragma unroll 4
+    for (int i = lane; i < batch; i += 64) {
+        const PagedSeq ls = paged_seq_lane(a, i);
+        if (token >= ls.first && token < ls.first + ls.lq) b = i;
+        tiles += (uint32_t)max(seq_tiles(a, ls), 0);
     }
-    if (b < 0) return;
+    const uint64_t at_lane = __ballot(b >= 0);
+    if (!at_lane) return;
+    b = __builtin_amdgcn_readlane(b, __builtin_ctzll(at_lane));
+    uint32_t u = 0x40000000u;
+    uint64_t slots = 0;
+    if (a.parts) {
+        u = piece_tiles(a, tiles, lane);
+#pragma unroll 4
+        for (int i = lane; i < b; i += 64) slots += seq_pieces(a, seq_work(a, paged_seq_lane(a, i), u)) >> 32;
+        slots = readlane64(wave_scan2(slots, lane), 63);
+    }
     const PagedSeq sq = paged_seq(a, b);
     const int qi = token - sq.first;
     if (qi >= min(sq.lq, a.max_q)) return;
@@ -172,7 +175,7 @@ static PagedPlan paged_plan(int32_t d, int32_t batch, int32_t total, int32_t q_h
     const int64_t cols = (int64_t)max_q * group, cus = paged_cus();
     // keys that a sequence's queries may see: the window's and the chunk's
     int64_t keys = max_kv;
-    if (wl >= 0) keys = std::min<int64_t>(keys, (int64_t)wl + max_q + std::max(wr, 0));
+    if (wl >= 0 && wr >= 0) keys = std::min<int64_t>(keys, (int64_t)wl + max_q + wr);
     // three blocks of 16 columns, four at D = 256 (16 sequences, FP8, bf16: D = 128, 4K keys, 32 columns 55 us
     // against the chunk kernel's 78, 48 columns 81 and 82, 64 columns 88 and 72; D = 256, up to 8K keys, 64
     // columns 99 and 107)
