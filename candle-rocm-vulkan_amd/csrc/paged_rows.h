@@ -637,7 +637,9 @@ __global__ __launch_bounds__(256, (VEC ? 4 : 1)) void paged_append_kernel(PagedR
 
 // Read-back of one side: y = scale * value(code) in f32, rounded to the output dtype; rows of holes
 // are zeros. The inverse of the append's split.
-template <int FMT, int D>
+// OUT: rows of whole 16-byte pieces of bf16 (1), f16 (2) or f32 (3); 0: any dtype and strides (all in one
+// kernel, their stores for every slot made a short call's instruction fetches its longest part).
+template <int FMT, int D, int OUT>
 __global__ __launch_bounds__(256) void paged_dequant_kernel(PagedRowsArgs a) {
     constexpr int LPR = D / 8, RPW = 64 / LPR;
     constexpr bool kB8 = FMT != CQKV_FMT_MXFP4;
@@ -720,14 +722,14 @@ __global__ __launch_bounds__(256) void paged_dequant_kernel(PagedRowsArgs a) {
             y[4] = p2.x * sc; y[5] = p2.y * sc; y[6] = p3.x * sc; y[7] = p3.y * sc;
         }
         const int64_t o = (row0 + s) * a.out_st + h * a.out_sh + e0;
-        if (a.out_vec && a.out_dtype == CQKV_F32) {
+        if constexpr (OUT == 3) {
             *(f32x4 *)((float *)a.out + o) = f32x4{y[0], y[1], y[2], y[3]};
             *(f32x4 *)((float *)a.out + o + 4) = f32x4{y[4], y[5], y[6], y[7]};
-        } else if (a.out_vec) {
+        } else if constexpr (OUT != 0) {
             u32x4 w;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                w[i] = a.out_dtype == CQKV_BF16 ? pack_bf16x2(y[2 * i], y[2 * i + 1]) : pack_f16x2(y[2 * i], y[2 * i + 1]);
+                w[i] = OUT == 1 ? pack_bf16x2(y[2 * i], y[2 * i + 1]) : pack_f16x2(y[2 * i], y[2 * i + 1]);
             *(u32x4 *)((uint16_t *)a.out + o) = w;
         } else {
 #pragma unroll
@@ -755,11 +757,18 @@ inline void launch_append_dim(int dk, int rope, dim3 grid, hipStream_t st, const
     else if (dk == 128) launch_append_rope<FMT, 128>(rope, grid, st, a);
     else launch_append_rope<FMT, 256>(rope, grid, st, a);
 }
+template <int FMT, int D>
+inline void launch_dequant_out(dim3 grid, hipStream_t st, const PagedRowsArgs &a) {
+    if (!a.out_vec) hipLaunchKernelGGL((paged_dequant_kernel<FMT, D, 0>), grid, dim3(256), 0, st, a);
+    else if (a.out_dtype == CQKV_BF16) hipLaunchKernelGGL((paged_dequant_kernel<FMT, D, 1>), grid, dim3(256), 0, st, a);
+    else if (a.out_dtype == CQKV_F16) hipLaunchKernelGGL((paged_dequant_kernel<FMT, D, 2>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((paged_dequant_kernel<FMT, D, 3>), grid, dim3(256), 0, st, a);
+}
 template <int FMT>
 inline void launch_dequant(int dk, dim3 grid, hipStream_t st, const PagedRowsArgs &a) {
-    if (dk == 64) hipLaunchKernelGGL((paged_dequant_kernel<FMT, 64>), grid, dim3(256), 0, st, a);
-    else if (dk == 128) hipLaunchKernelGGL((paged_dequant_kernel<FMT, 128>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((paged_dequant_kernel<FMT, 256>), grid, dim3(256), 0, st, a);
+    if (dk == 64) launch_dequant_out<FMT, 64>(grid, st, a);
+    else if (dk == 128) launch_dequant_out<FMT, 128>(grid, st, a);
+    else launch_dequant_out<FMT, 256>(grid, st, a);
 }
 
 // Per-format launchers, defined in paged_inst.hip.
