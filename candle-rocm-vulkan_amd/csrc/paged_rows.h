@@ -11,8 +11,8 @@
 // and the eight tokens' loads are in flight together. A lane then holds the 8 x 8 block of codes that
 // is 64 (or 32) contiguous bytes of a value tile: the transpose is byte permutes in registers, with no
 // LDS and no barrier. Bound by HBM; single tokens by the latency of the chain sequence -> page -> row. 8192 tokens into MXFP4, 8 kv heads of
-// 128: 13.6 us (3.3 TB/s of rows and codes); 6333 tokens rotated on three axes into FP8, 32 / 8 heads: 39 us
-// (3.9 TB/s); 48769 rows of one FP8 side read back: 30 us (5.0 TB/s); 64 single tokens: 4.9 us.
+// 128: 13 us (3.3 TB/s of rows and codes); 6333 tokens rotated on three axes into FP8, 32 / 8 heads: 39 us
+// (3.9 TB/s); 48769 rows of one FP8 side read back: 24 us (6.2 TB/s); 64 single tokens: 4.9 us.
 #pragma once
 
 #include <type_traits>
@@ -722,15 +722,16 @@ __global__ __launch_bounds__(256) void paged_dequant_kernel(PagedRowsArgs a) {
             y[4] = p2.x * sc; y[5] = p2.y * sc; y[6] = p3.x * sc; y[7] = p3.y * sc;
         }
         const int64_t o = (row0 + s) * a.out_st + h * a.out_sh + e0;
+        // (nontemporal: 48769 rows of two FP8 sides 62 us, 66 with cached stores)
         if constexpr (OUT == 3) {
-            *(f32x4 *)((float *)a.out + o) = f32x4{y[0], y[1], y[2], y[3]};
-            *(f32x4 *)((float *)a.out + o + 4) = f32x4{y[4], y[5], y[6], y[7]};
+            __builtin_nontemporal_store(f32x4{y[0], y[1], y[2], y[3]}, (f32x4 *)((float *)a.out + o));
+            __builtin_nontemporal_store(f32x4{y[4], y[5], y[6], y[7]}, (f32x4 *)((float *)a.out + o + 4));
         } else if constexpr (OUT != 0) {
             u32x4 w;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 w[i] = OUT == 1 ? pack_bf16x2(y[2 * i], y[2 * i + 1]) : pack_f16x2(y[2 * i], y[2 * i + 1]);
-            *(u32x4 *)((uint16_t *)a.out + o) = w;
+            __builtin_nontemporal_store(w, (u32x4 *)((uint16_t *)a.out + o));
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)

@@ -67,7 +67,7 @@ static int append_run(const char *who, const cqkv_side *k, int rope, PagedRowsAr
     const int64_t tiles = tiles_bound(a.pt.total, a.pt.batch);
     // with angles: half a tile for a wavefront, and two head groups where that leaves 4 wavefronts to every
     // SIMD (6333 tokens, FP8, 32 / 8 heads, D = 128: append and read-back 63 us with one group, 59 with two,
-    // 60 with three, 68 with four)
+    // 60 with three, 68 with four, before the read-back's stores were nontemporal)
     const int64_t kq = a.k_units + a.q_units, parts = rope ? 2 : 1;
     a.per = rope && tiles * parts * kq >= 8192 ? 2 : 1;
     a.units = (int)(parts * ((kq + a.per - 1) / a.per) + a.v_units);
